@@ -27,7 +27,8 @@ LIB = os.path.join(PKG, "libbsi_b200.so")
 EXT_SUFFIX = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
 EXT = os.path.join(PKG, "bsi_ops" + EXT_SUFFIX)
 
-CUDA_SOURCES = ["common.cu", "pack.cu", "ewah.cu", "dot.cu", "dot_tcgen05.cu", "dot_decode.cu", "dot_bmma.cu", "peer.cu"]
+CUDA_SOURCES = ["common.cu", "pack.cu", "ewah.cu", "dot.cu", "dot_tcgen05.cu", "dot_decode.cu", "dot_bmma.cu", "peer.cu", "vocab.cu"]
+EXT_SOURCES = ["bsi_ops_module.cpp", "lm_ops.cpp"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
 
@@ -97,9 +98,9 @@ def build_ext(verbose: bool = False) -> str:
     import torch
     from torch.utils import cpp_extension as ce
 
-    src = os.path.join(CSRC, "bsi_ops_module.cpp")
+    srcs = [os.path.join(CSRC, n) for n in EXT_SOURCES]
     stamp = os.path.join(OBJ, "bsi_ops.stamp")
-    want = _hash([src, os.path.join(ROOT, "include", "bsi_b200.h")], torch.__version__ + EXT_SUFFIX)
+    want = _hash(srcs + [os.path.join(CSRC, "lm_ops.h"), os.path.join(ROOT, "include", "bsi_b200.h")], torch.__version__ + EXT_SUFFIX)
     if _stamp_ok(stamp, want, EXT):
         return EXT
     os.makedirs(OBJ, exist_ok=True)
@@ -112,7 +113,7 @@ def build_ext(verbose: bool = False) -> str:
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            "-DTORCH_EXTENSION_NAME=bsi_ops", "-DTORCH_API_INCLUDE_EXTENSION_H",
            f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-Wno-attributes"] + inc + [
-           src, "-o", EXT,
+           *srcs, "-o", EXT,
            "-L" + PKG, "-lbsi_b200", "-Wl,-rpath,$ORIGIN",
            "-L" + torch_lib, "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_cuda", "-lc10_cuda", "-ltorch_python",
            "-Wl,-rpath," + torch_lib]

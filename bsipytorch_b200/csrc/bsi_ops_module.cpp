@@ -36,6 +36,7 @@
 #include <vector>
 
 #include "bsi_b200.h"
+#include "lm_ops.h"
 
 namespace py = pybind11;
 
@@ -1797,4 +1798,5 @@ PYBIND11_MODULE(bsi_ops, m) {
           "Load a key set written by save_keyset; returns (capsule, total_mem_bytes, num_keys, d, W)");
     m.def("keyset_size_on_disk", &keyset_size_on_disk, py::arg("keyset_cuda_cap"), "Return (mem_in_memory, bytes_on_disk)");
     m.def("device_status", &device_status, "Read and clear the device-side timeout status word (synchronises)");
+    register_lm_ops(m);
 }

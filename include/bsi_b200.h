@@ -438,6 +438,53 @@ int bsi_b200_ewah_encode_static(const uint64_t* words, int64_t S, int64_t W, dou
 int bsi_b200_cast_bias(const float* out, int64_t ldo, const float* bias, int64_t Q, int64_t R,
                        void* y, int64_t ldy, int y_dtype, bsi_stream_t stream);
 
+/* ---- what a model answers, and how near it is to a teacher ---------------------------------------------------------------
+ * Operators over rows of logits, V each with a stride of one; dtype BSI_DTYPE_*. The reference judges its layers by argmaxes of
+ * torch's (benchmark_performance_bsi.py:209-217); it has no counterpart of these.
+ *
+ * Where row r of a 2-D or 3-D tensor starts, in elements: per == 0: r * row_stride; else
+ * (r / per) * block_stride + (r % per) * row_stride, as for logits[:, :-1] of a [batch, length, V] tensor. */
+typedef struct bsi_row_plan {
+    int64_t per, block_stride, row_stride;
+} bsi_row_plan;
+
+/* For each row z and its token t (tokens NULL: none): logprobs = log softmax(z)[t], ranks = how many entries are larger, or equal at
+ * a lower index (0: the argmax), entropy = -sum p log p, and the `top` largest entries, their log probabilities and indices, equal
+ * values by ascending index. top at most 128 and V. A token outside [0, V) is not scored: logprob 0, rank -1. A row that holds a NaN or
+ * +inf, or nothing but -inf, has NaN for its log probabilities and entropy; its rank means nothing. logprobs, ranks and entropy may
+ * be NULL. All outputs are contiguous, [rows] and [rows, top]. */
+int bsi_b200_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan,
+                            const int64_t* tokens, const bsi_row_plan* token_plan, int top,
+                            float* logprobs, int64_t* ranks, float* entropy, float* top_logprobs, int64_t* top_ids,
+                            bsi_stream_t stream);
+
+/* Distillation from a teacher's K top entries a row (ids and teacher [rows, K], 1 to 512), with q = softmax(z / temperature):
+ *   tail 0: teacher holds logits, p = softmax over the listed ones of t / temperature, loss = T^2 sum p (log p - log q)
+ *   tail 1: teacher holds log probabilities at this temperature, p = exp(t); what they leave, rest = max(0, 1 - sum p), stands for all
+ *           that is not listed: loss = T^2 [sum p (log p - log q) + rest (log rest - log q_rest)]
+ * Entries with an id outside [0, V) are not there; an id listed twice counts with the sum of its probabilities. A row's loss is
+ * multiplied by weights[r] (float32, NULL: 1); a row of weight 0 is not read, its loss and gradient are 0. loss: the sum over the rows,
+ * mean != 0: divided by the weights' sum (0 where that is 0), which weight_sum receives. row_loss [rows]: the rows' weighted losses.
+ * saved [rows, 4] float32, 16-byte aligned: what the backward pass takes. loss, weight_sum and saved may be NULL. */
+int bsi_b200_distill_forward(const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan,
+                             const int64_t* ids, const void* teacher, int teacher_dtype, int K, float temperature, int tail,
+                             const float* weights, int mean, float* row_loss, float* saved, float* loss, float* weight_sum,
+                             bsi_stream_t stream);
+/* grad [rows, V] in the logits' type, rows grad_stride >= V apart, not overlapping the logits:
+ * upstream[r * upstream_stride] * weights[r] / *denominator * dloss_r/dz. upstream and denominator may be NULL (1); a denominator of 0
+ * gives a gradient of 0. */
+int bsi_b200_distill_backward(const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan,
+                              const int64_t* ids, const void* teacher, int teacher_dtype, int K, float temperature, int tail,
+                              const float* weights, const float* saved, const float* upstream, int64_t upstream_stride,
+                              const float* denominator, void* grad, int64_t grad_stride, bsi_stream_t stream);
+/* Both at once, the logits read once: a row stays in the shared memory of the CTAs that share it. Same loss, and the gradient of
+ * `loss`. For rows that fit (host function, 1 or 0: about 390,000 float32 or 780,000 16-bit logits). loss and weight_sum are needed. */
+int bsi_b200_distill_fused_fits(int dtype, int64_t V, int tail);
+int bsi_b200_distill_fused(const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan,
+                           const int64_t* ids, const void* teacher, int teacher_dtype, int K, float temperature, int tail,
+                           const float* weights, int mean, float* row_loss, float* loss, float* weight_sum,
+                           void* grad, int64_t grad_stride, bsi_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
