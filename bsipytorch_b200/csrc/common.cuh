@@ -94,6 +94,8 @@ bool pdl_enabled();
 
 // Reads and clears the status word of the peer barrier kernels (0 = clean, 64 + p = gave up waiting for rank p).
 int take_peer_status(int* v);
+// The same of the 4-bit products' bounded waits (129 and up).
+int take_fp4_status(int* v);
 
 // For kernels that start while the kernels in front of them on the stream still run (programmatic dependent launch): the
 // pointer, behind griddepcontrol.wait, to something those may have written. Loads through it are ordinary coherent ones

@@ -1,5 +1,5 @@
-// Host side of the operators around a language model's logits (token log probabilities, distillation), as functions
-// of the `bsi_ops` module. Checks, row plans and allocations; every kernel lives in libbsi_b200.so.
+// Host side of the operators around a language model's logits (token log probabilities, distillation) and of the 4-bit linear
+// layers, as functions of the `bsi_ops` module. Checks, row plans and allocations; every kernel lives in libbsi_b200.so.
 #include "lm_ops.h"
 
 #include <torch/extension.h>
@@ -213,9 +213,127 @@ bool distill_fused_fits(const torch::Tensor& logits, bool tail) {
     return bsi_b200_distill_fused_fits(dtype_code(logits, "logits"), logits.size(-1), tail ? 1 : 0) == 1;
 }
 
+// ---- microscaled 4-bit floating point ----------------------------------------------------------------------------------------
+
+// The tensors of a packed matrix: codes [rows, ld] uint8, scales uint8, row_scale [rows] float32 (nvfp4) or undefined.
+struct Fp4 {
+    at::Tensor codes, scales, row_scale;
+    int64_t rows, K;
+    int format;
+
+    const float* row() const { return row_scale.defined() ? row_scale.data_ptr<float>() : nullptr; }
+
+    // Nothing but room.
+    Fp4(int64_t r, int64_t k, int f, at::Device dev) : rows(r), K(k), format(f) {
+        codes = fresh({rows, (K + 31) / 32 * 16}, at::kByte, dev);
+        scales = fresh({bsi_b200_fp4_scale_bytes(rows, K, format)}, at::kByte, dev);
+        if (format == BSI_FP4_NV) row_scale = fresh({rows}, at::kFloat, dev);
+    }
+    // A matrix that a caller holds.
+    Fp4(const at::Tensor& c, const at::Tensor& s, const OptTensor& g, int64_t k, int f) : codes(c), scales(s), rows(c.size(0)), K(k), format(f) {
+        TORCH_CHECK(f == BSI_FP4_MX || f == BSI_FP4_NV, "unknown 4-bit format ", f);
+        TORCH_CHECK(c.is_cuda() && c.dim() == 2 && c.scalar_type() == at::kByte && c.is_contiguous() && k >= 1 && c.size(1) == (k + 31) / 32 * 16,
+                    "codes must be a contiguous uint8 CUDA tensor [rows, ", (k + 31) / 32 * 16, "]");
+        TORCH_CHECK(s.device() == c.device() && s.scalar_type() == at::kByte && s.is_contiguous() && s.numel() == bsi_b200_fp4_scale_bytes(rows, k, f),
+                    "scales must be ", bsi_b200_fp4_scale_bytes(rows, k, f), " bytes on the codes' device");
+        TORCH_CHECK(g.has_value() == (f == BSI_FP4_NV), "nvfp4 matrices, and only they, have row scales");
+        if (g.has_value()) {
+            TORCH_CHECK(g->device() == c.device() && g->scalar_type() == at::kFloat && g->is_contiguous() && g->numel() == rows, "one float32 row scale per row");
+            row_scale = *g;
+        }
+    }
+};
+
+void quantize_into(const at::Tensor& x2d, Fp4& to) {
+    check_status(bsi_b200_fp4_quantize(x2d.data_ptr(), dtype_code(x2d, "x"), to.rows, to.K, to.rows > 1 ? x2d.stride(0) : to.K, to.format,
+                                       to.codes.data_ptr<uint8_t>(), to.codes.size(1), to.scales.data_ptr<uint8_t>(),
+                                       to.row_scale.defined() ? to.row_scale.data_ptr<float>() : nullptr, current_stream()),
+                 "bsi_b200_fp4_quantize");
+}
+
+at::Tensor as_rows(const at::Tensor& given, const char* what) {
+    at::Tensor t = given.detach();
+    TORCH_CHECK(t.is_cuda(), what, " must be a CUDA tensor: there is no CPU path");
+    TORCH_CHECK(t.dim() >= 1 && t.size(-1) >= 1, what, " must be [..., features]");
+    dtype_code(t, what);
+    if (t.dim() != 2) t = t.reshape({t.numel() / t.size(-1), t.size(-1)});
+    // rows may lie further apart than they are long, elements not
+    if ((t.size(1) > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < t.size(1))) t = t.contiguous();
+    return t;
+}
+
+py::tuple fp4_quantize(const torch::Tensor& x, int format) {
+    const at::Tensor t = as_rows(x, "x");
+    TORCH_CHECK(format == BSI_FP4_MX || format == BSI_FP4_NV, "unknown 4-bit format ", format);
+    c10::cuda::CUDAGuard guard(t.device());
+    Fp4 q(t.size(0), t.size(1), format, t.device());
+    quantize_into(t, q);
+    return py::make_tuple(q.codes, q.scales, q.row_scale.defined() ? py::cast(q.row_scale) : py::none());
+}
+
+at::Tensor fp4_dequantize(const torch::Tensor& codes, const torch::Tensor& scales, const OptTensor& row_scale, int64_t K, int format, py::object dtype) {
+    const Fp4 q(codes, scales, row_scale, K, format);
+    c10::cuda::CUDAGuard guard(codes.device());
+    at::Tensor out = fresh({q.rows, K}, torch::python::detail::py_object_to_dtype(dtype), codes.device());
+    check_status(bsi_b200_fp4_dequantize(q.codes.data_ptr<uint8_t>(), q.codes.size(1), q.scales.data_ptr<uint8_t>(), q.row(), q.rows, K, format, out.data_ptr(),
+                                         dtype_code(out, "dtype"), K, current_stream()),
+                 "bsi_b200_fp4_dequantize");
+    return out;
+}
+
+// The bias as the product reads it. A cast of its own has to stand in front of the packer, behind which the product starts early.
+at::Tensor bias_of(const OptTensor& bias, const Fp4& w) {
+    if (!bias.has_value()) return at::Tensor();
+    TORCH_CHECK(bias->device() == w.codes.device() && bias->numel() == w.rows, "one bias per output, on the weights' device");
+    return bias->detach().to(at::kFloat).contiguous();
+}
+
+at::Tensor product(const Fp4& x, const Fp4& w, const at::Tensor& bias, bool relu, at::ScalarType type, bool behind_packer) {
+    TORCH_CHECK(x.K == w.K, "activations of ", x.K, " features, weights of ", w.K);
+    TORCH_CHECK(x.format == w.format, "activations and weights are packed in different 4-bit formats");
+    TORCH_CHECK(x.codes.device() == w.codes.device(), "activations and weights live on different devices");
+    at::Tensor y = fresh({x.rows, w.rows}, type, w.codes.device());
+    check_status(bsi_b200_fp4_linear(x.codes.data_ptr<uint8_t>(), x.codes.size(1), x.scales.data_ptr<uint8_t>(), x.row(), w.codes.data_ptr<uint8_t>(),
+                                     w.codes.size(1), w.scales.data_ptr<uint8_t>(), w.row(),
+                                     bias.defined() ? bias.data_ptr<float>() : nullptr, x.rows, w.rows, w.K, w.format, y.data_ptr(), w.rows,
+                                     dtype_code(y, "the output"), relu ? BSI_ACT_RELU : BSI_ACT_NONE, behind_packer ? 1 : 0,
+                                     current_stream()),
+                 "bsi_b200_fp4_linear");
+    return y;
+}
+
+at::Tensor fp4_linear(const torch::Tensor& x, const torch::Tensor& codes, const torch::Tensor& scales, const OptTensor& row_scale, int64_t K, int format,
+                      const OptTensor& bias, bool relu, const c10::optional<py::object>& dtype) {
+    const Fp4 w(codes, scales, row_scale, K, format);
+    const at::Tensor t = as_rows(x, "x");
+    TORCH_CHECK(t.size(1) == K, "activations of ", t.size(1), " features, weights of ", K);
+    TORCH_CHECK(t.device() == codes.device(), "activations and weights live on different devices");
+    c10::cuda::CUDAGuard guard(t.device());
+    const at::Tensor b = bias_of(bias, w);
+    Fp4 q(t.size(0), K, format, t.device());
+    quantize_into(t, q);
+    at::Tensor y = product(q, w, b, relu, dtype.has_value() ? torch::python::detail::py_object_to_dtype(*dtype) : x.scalar_type(), true);
+    if (x.dim() != 2) y = y.view(with_last(x.sizes().slice(0, x.dim() - 1), w.rows));
+    return y;
+}
+
+at::Tensor fp4_linear_packed(const torch::Tensor& xc, const torch::Tensor& xs, const OptTensor& xg, const torch::Tensor& codes, const torch::Tensor& scales,
+                             const OptTensor& row_scale, int64_t K, int x_format, int format, const OptTensor& bias, bool relu, py::object dtype) {
+    const Fp4 w(codes, scales, row_scale, K, format), q(xc, xs, xg, K, x_format);
+    c10::cuda::CUDAGuard guard(codes.device());
+    return product(q, w, bias_of(bias, w), relu, torch::python::detail::py_object_to_dtype(dtype), false);
+}
+
 }  // namespace
 
 void register_lm_ops(py::module& m) {
+    m.def("fp4_quantize", &fp4_quantize, py::arg("x"), py::arg("format"), "(codes, scales, row scales or None) of a matrix in a 4-bit format");
+    m.def("fp4_dequantize", &fp4_dequantize, py::arg("codes"), py::arg("scales"), py::arg("row_scale"), py::arg("features"), py::arg("format"),
+          py::arg("dtype"));
+    m.def("fp4_linear", &fp4_linear, py::arg("x"), py::arg("codes"), py::arg("scales"), py::arg("row_scale"), py::arg("features"), py::arg("format"),
+          py::arg("bias"), py::arg("relu"), py::arg("dtype") = py::none(), "Pack x, then the product with a packed weight");
+    m.def("fp4_linear_packed", &fp4_linear_packed, py::arg("x_codes"), py::arg("x_scales"), py::arg("x_row_scale"), py::arg("codes"), py::arg("scales"),
+          py::arg("row_scale"), py::arg("features"), py::arg("x_format"), py::arg("format"), py::arg("bias"), py::arg("relu"), py::arg("dtype"));
     m.def("token_logprobs", &token_logprobs, py::arg("logits"), py::arg("tokens") = py::none(), py::arg("top_k") = 0,
           "(logprobs, ranks, entropy, top_logprobs, top_ids) of rows of logits");
     m.def("distill_forward", &distill_forward, py::arg("logits"), py::arg("ids"), py::arg("teacher"), py::arg("temperature"), py::arg("tail"),

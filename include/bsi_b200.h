@@ -485,6 +485,35 @@ int bsi_b200_distill_fused(const void* logits, int dtype, int64_t rows, int64_t 
                            const float* weights, int mean, float* row_loss, float* loss, float* weight_sum,
                            void* grad, int64_t grad_stride, bsi_stream_t stream);
 
+/* ---- microscaled 4-bit floating point ------------------------------------------------------------------------------------
+ * A second number format for the linear layers (the reference has none of the kind): e2m1 elements, two to a byte, under block scales.
+ *   BSI_FP4_MX  blocks of 32 along a row, scale 2^(floor(log2 amax) - 2) (e8m0), quotients beyond 6 saturate. A block that holds an
+ *               infinity or a NaN stands for NaN.
+ *   BSI_FP4_NV  blocks of 16, scale e4m3(amax / (6 g)) under a power of two g per row, the smallest with 2688 g >= the row's largest
+ *               magnitude (at least 2^-100; 1 for zeros). row_scale [rows] float32 receives g; a row that holds an infinity or a NaN
+ *               gets NaN, and stands for NaN.
+ * Elements round to the nearest value, ties to the even code.
+ * codes: [rows, ld] bytes, ld a multiple of 16 and at least ceil(K / 32) * 16, zero behind column K. scales: 512 bytes for 128 rows x 4
+ * consecutive blocks (row r % 32 at 16 bytes each, then r / 32 % 4 at 4 bytes, then the block), tiles of a row tile behind one
+ * another, bsi_b200_fp4_scale_bytes in all (-1 for bad arguments). Both 16-byte aligned. row_scale may be NULL for BSI_FP4_MX. */
+#define BSI_FP4_MX 0
+#define BSI_FP4_NV 1
+int64_t bsi_b200_fp4_scale_bytes(int64_t rows, int64_t K, int format);
+int bsi_b200_fp4_quantize(const void* x, int dtype, int64_t rows, int64_t K, int64_t ldx, int format, uint8_t* codes, int64_t ld,
+                          uint8_t* scales, float* row_scale, bsi_stream_t stream);
+/* The values that such a matrix stands for, rounded once to dtype. */
+int bsi_b200_fp4_dequantize(const uint8_t* codes, int64_t ld, const uint8_t* scales, const float* row_scale, int64_t rows, int64_t K,
+                            int format, void* out, int dtype, int64_t ldo, bsi_stream_t stream);
+/* y[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) of two matrices packed in the same format, x [M, K] and w [N, K]: products and block
+ * scales on the tensor cores, float32 sums, one rounding to y_dtype. bias float32 [N] or NULL; activation BSI_ACT_*. row scales are
+ * factors of any float32 value. behind_packer != 0: the launch right before this one on the stream is the
+ * bsi_b200_fp4_quantize that writes x, and nothing that may still run writes w: w is then read while x is still being packed. A wait
+ * that gives up shows in bsi_b200_device_status as 129 to 131. */
+int bsi_b200_fp4_linear(const uint8_t* x_codes, int64_t ldx, const uint8_t* x_scales, const float* x_row_scale,
+                        const uint8_t* w_codes, int64_t ldw, const uint8_t* w_scales, const float* w_row_scale, const float* bias,
+                        int64_t M, int64_t N, int64_t K, int format, void* y, int64_t ldy, int y_dtype, int activation, int behind_packer,
+                        bsi_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
