@@ -96,6 +96,8 @@ bool pdl_enabled();
 int take_peer_status(int* v);
 // The same of the 4-bit products' bounded waits (129 and up).
 int take_fp4_status(int* v);
+// The same of the kernels over rows of logits (144).
+int take_vocab_status(int* v);
 
 // For kernels that start while the kernels in front of them on the stream still run (programmatic dependent launch): the
 // pointer, behind griddepcontrol.wait, to something those may have written. Loads through it are ordinary coherent ones

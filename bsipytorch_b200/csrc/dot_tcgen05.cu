@@ -824,6 +824,8 @@ extern "C" int bsi_b200_device_status(int* status_out) {
     if (v == 0) v = pv;
     if (int rc = take_fp4_status(&pv)) return rc;
     if (v == 0) v = pv;
+    if (int rc = take_vocab_status(&pv)) return rc;
+    if (v == 0) v = pv;
     *status_out = v;
     return BSI_OK;
 }

@@ -209,10 +209,6 @@ py::tuple distill_fused(const torch::Tensor& logits, const torch::Tensor& given_
     return py::make_tuple(reduction == kNone ? row_loss : loss, grad);
 }
 
-bool distill_fused_fits(const torch::Tensor& logits, bool tail) {
-    return bsi_b200_distill_fused_fits(dtype_code(logits, "logits"), logits.size(-1), tail ? 1 : 0) == 1;
-}
-
 // ---- microscaled 4-bit floating point ----------------------------------------------------------------------------------------
 
 // The tensors of a packed matrix: codes [rows, ld] uint8, scales uint8, row_scale [rows] float32 (nvfp4) or undefined.
@@ -342,5 +338,4 @@ void register_lm_ops(py::module& m) {
           py::arg("weights"), py::arg("saved"), py::arg("upstream"), py::arg("weight_sum"), "The logits' gradient");
     m.def("distill_fused", &distill_fused, py::arg("logits"), py::arg("ids"), py::arg("teacher"), py::arg("temperature"), py::arg("tail"),
           py::arg("weights"), py::arg("reduction"), "(loss, the logits' gradient) with the logits read once");
-    m.def("distill_fused_fits", &distill_fused_fits, py::arg("logits"), py::arg("tail"));
 }

@@ -7,36 +7,60 @@
 #include "vocab.cuh"
 
 namespace bsi {
+
+__device__ int g_vocab_status = 0;
+
+int take_vocab_status(int* v) {
+    int s = 0;
+    BSI_CUDA_TRY(cudaMemcpyFromSymbol(&s, g_vocab_status, sizeof(int)));
+    if (s != 0) {
+        const int zero = 0;
+        BSI_CUDA_TRY(cudaMemcpyToSymbol(g_vocab_status, &zero, sizeof(int)));
+    }
+    *v = s;
+    return BSI_OK;
+}
+
 namespace {
 
 namespace cg = cooperative_groups;
+using vocab::kBatch;
+using vocab::kChunk;
 using vocab::kThreads;
 using vocab::kWarps;
 using vocab::Piece;
+using vocab::Ring;
 using vocab::RowPlan;
 using vocab::Span;
 using vocab::Stats;
 
-constexpr int kBatch = 4;               // 16-byte pieces that a thread has under way
 constexpr int kMaxTop = 128;            // alternatives of token_logprobs
-constexpr int kCandidates = 2048;       // entries at least as large as the block's bound that it keeps
+constexpr int kCandidates = 1024;       // entries at least as large as the bound of their time that a block keeps
+constexpr int kSorted = 64;             // above so many they are thinned out by the last bound before they are put in order
+constexpr int kPerSm = 3;               // CTAs of 256 threads with 80 registers
+constexpr int kStages = 2;              // chunks under way in each: 96 KB an SM, 6.2 TB/s where nothing but the statistics is computed
 constexpr int kMaxListed = 512;         // teacher entries per row
+static_assert(vocab::kMaxCluster * kMaxTop <= kCandidates, "CTA 0 gathers the others' lists where its candidates were");
 
 // ---- log probabilities, ranks, entropy, top alternatives ---------------------------------------------------------------------
 //
 // For a row z and a token t:  logprob = z_t - lse,  lse = m + log sum exp(z - m),  entropy = lse - sum p z,
 // rank = #{z_j > z_t} + #{j < t, z_j = z_t}, top = the k largest, equal values by ascending index.
 //
-// The top k ride on the same pass. The largest value that each thread met is its running maximum; with B the k-th largest of those
-// 512 maxima, at least k entries are >= B, so the k largest all are, and few others. A search over the upper 16 bits of the ordered
-// maxima (16 votes of the block) finds a B that is no larger; only threads whose maximum reaches it look at their pieces again
-// (out of L2), and the entries found are put in order by counting for each one how many come before it.
-// Where more than kCandidates entries reach B (a row that is -inf but for a few, a constant row), the block selects by radix: four
-// passes over 8 bits each give the k-th value, one pass the larger entries, one in index order the equal ones.
+// The top k ride on the same pass. Every warp knows the j-th largest of its lanes' running maxima, j = ceil(k / 8); with B the t-th
+// largest of these over the 8 warps, t = ceil(k / j), at least k entries are >= B, so the k largest all are, and few others. The bound
+// is found behind the first chunk, which the threads still hold (one barrier), and again behind chunks 2, 4, 8, ... without one: any
+// bound of an earlier time is one. Entries that reach the bound of their time are kept (about k for each doubling of what was read), and put in order at the end by
+// counting for each one how many come before it. Reading a row again where a thread's maximum reaches the final bound costs a quarter of
+// the row from memory at k = 64 (633 x 128011 float32: 163 us).
+// Where more than kCandidates entries are kept (a row in ascending order, a constant one), the block selects by radix: four passes over
+// 8 bits each give the k-th value, one pass the larger entries, one in index order the equal ones. -inf is kept only where a row has
+// fewer than k other entries.
 
 struct ScoreArgs {
     const void* logits;
     RowPlan rows;
+    uint32_t count;      // rows
     int64_t V;
     const int64_t* tokens;
     RowPlan tokens_at;
@@ -54,15 +78,56 @@ struct ScoreShared {
     Stats mine;          // this CTA's part of the row, read by CTA 0
     int ahead;
     int found;           // candidates
+    int lengths[vocab::kMaxCluster];      // CTA 0: the others' `listed`
     int listed;          // entries in `best`: min(top, elements of this part)
+    volatile uint32_t bound[kWarps];      // the warps' own
+    uint32_t agreed_bound;                // the highest that has come of them
+    uint64_t bars[2 * kStages];
+    vocab::Feed feed;
     uint32_t hist[256];
     uint32_t prefix, need;
     unsigned long long best[kMaxTop];      // this CTA's largest, in order
     unsigned long long cand[kCandidates];
+
+    // The t-th largest of the voting warps' bounds, by whole warps. Equal ones by their number, so that each has a rank of its own.
+    __device__ __forceinline__ uint32_t agreed(int voters, int t) const {
+        const int lane = threadIdx.x & 31;
+        const uint32_t own = lane < voters ? bound[lane] * kWarps + static_cast<uint32_t>(lane) : 0u;
+        int rank = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) rank += __shfl_sync(0xFFFFFFFFu, own, w) > own;
+        const unsigned it = __ballot_sync(0xFFFFFFFFu, lane < voters && rank == t - 1);
+        return it == 0u ? 0u : __shfl_sync(0xFFFFFFFFu, own, __ffs(it) - 1) / kWarps;
+    }
 };
 
 __device__ __forceinline__ unsigned long long sort_key(float v, int64_t index) {
     return (static_cast<unsigned long long>(vocab::ordered(v)) << 32) | static_cast<uint32_t>(~static_cast<uint32_t>(index));
+}
+
+// The first `need` entries of [lo, hi), in index order, whose place in the order is `prefix`, into sh.cand[at ..). All threads.
+template <typename T>
+__device__ void take_equal(ScoreShared& sh, const T* row, int64_t lo, int64_t hi, uint32_t prefix, int at, int need) {
+    int taken = 0;
+    for (int64_t i0 = lo; i0 < hi && taken < need; i0 += kThreads) {
+        const int64_t i = i0 + threadIdx.x;
+        const float v = i < hi ? Piece<T>::one(row[i]) : 0.0f;
+        const bool eq = i < hi && vocab::ordered(v) == prefix;
+        const unsigned votes = __ballot_sync(0xFFFFFFFFu, eq);
+        if ((threadIdx.x & 31) == 0) sh.warp_ahead[threadIdx.x >> 5] = __popc(votes);
+        __syncthreads();
+        int before = 0, all = 0;
+        for (int w = 0; w < kWarps; ++w) {
+            const int n = sh.warp_ahead[w];
+            if (w < static_cast<int>(threadIdx.x >> 5)) before += n;
+            all += n;
+        }
+        const int place = taken + before + __popc(votes & ((1u << (threadIdx.x & 31)) - 1u));
+        if (eq && place < need) sh.cand[at + place] = sort_key(v, i);
+        taken += all;
+        __syncthreads();
+    }
+    __syncthreads();
 }
 
 // The exact k largest of [lo, hi) into sh.cand[0 .. k), in no order, for any contents. All threads; k <= hi - lo.
@@ -101,102 +166,180 @@ __device__ void select_by_radix(ScoreShared& sh, const T* row, int64_t lo, int64
         if (vocab::ordered(v) > prefix) sh.cand[atomicAdd(&sh.found, 1)] = sort_key(v, i);
     }
     __syncthreads();
-    int taken = 0;
-    for (int64_t i0 = lo; i0 < hi && taken < need; i0 += kThreads) {
-        const int64_t i = i0 + threadIdx.x;
-        const float v = i < hi ? Piece<T>::one(row[i]) : 0.0f;
-        const bool eq = i < hi && vocab::ordered(v) == prefix;
-        const unsigned votes = __ballot_sync(0xFFFFFFFFu, eq);
-        if ((threadIdx.x & 31) == 0) sh.warp_ahead[threadIdx.x >> 5] = __popc(votes);
-        __syncthreads();
-        int before = 0, all = 0;
-        for (int w = 0; w < kWarps; ++w) {
-            const int n = sh.warp_ahead[w];
-            if (w < static_cast<int>(threadIdx.x >> 5)) before += n;
-            all += n;
-        }
-        const int place = taken + before + __popc(votes & ((1u << (threadIdx.x & 31)) - 1u));
-        if (eq && place < need) sh.cand[(k - need) + place] = sort_key(v, i);
-        taken += all;
-        __syncthreads();
-    }
-    __syncthreads();
+    take_equal<T>(sh, row, lo, hi, prefix, k - need, need);
 }
 
+// The j-th largest of a warp's places, by halving: the largest place that at least j lanes reach (0: none is).
+__device__ __forceinline__ uint32_t warp_bound(uint32_t place, int j) {
+    if (j == 1) return __reduce_max_sync(0xFFFFFFFFu, place);
+    uint32_t bound = 0;
+#pragma unroll 4
+    for (int bit = 15; bit >= 0; --bit) {
+        const uint32_t tryit = bound | (1u << bit);
+        if (__popc(__ballot_sync(0xFFFFFFFFu, place >= tryit)) >= j) bound = tryit;
+    }
+    return bound;
+}
+
+// The row's ends and the few pieces of a CTA's last round go one by one; the rest in batches.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) score_kernel(const ScoreArgs a) {
+struct ScoreThread {
+    vocab::Running<T, true> run;
+    int ahead;
+    uint32_t at, behind;       // thresholds in front of the token's piece and from it on, as words
+    int token_piece;
+    float bound;               // of the entries that are kept, and as a word
+    uint32_t thr;
+
+    __device__ __forceinline__ void set_bound(uint32_t place) {
+        const T b = Piece<T>::smallest(max(place, Piece<T>::kFloor));
+        bound = Piece<T>::one(b);
+        thr = Piece<T>::word(b);
+    }
+
+    template <int B>
+    __device__ __forceinline__ float take(const uint4 (&u)[B], int v) {
+        const float top = run.take(u, vocab::kLog2e);
+        typename Piece<T>::Count count;
+#pragma unroll
+        for (int b = 0; b < B; ++b) count.add(u[b], v + b * kThreads < token_piece ? at : behind);
+        ahead += count.total();
+        return top;
+    }
+    // Keeps the entries that reach the bound; top: the largest of them all, from: where the pieces lie, kThreads pieces apart.
+    template <int B>
+    __device__ __forceinline__ void keep(ScoreShared& sh, const Span<T>& span, const uint4 (&u)[B], int v, float top, const T* from) {
+        if (top < bound) return;
+        uint32_t reached = 0;
+#pragma unroll
+        for (int b = 0; b < B; ++b) reached |= Piece<T>::reach(u[b], thr) << (b * Piece<T>::kVec);
+        while (reached != 0u) {
+            const int bit = __ffs(reached) - 1;
+            reached &= reached - 1u;
+            const int off = bit / Piece<T>::kVec * kThreads * Piece<T>::kVec + bit % Piece<T>::kVec, i = span.element(v) + off;
+            if (i < 0 || i >= span.V) continue;
+            const int place = atomicAdd(&sh.found, 1);
+            if (place < kCandidates) sh.cand[place] = sort_key(Piece<T>::one(from[off]), i);
+        }
+    }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, kPerSm) score_kernel(const ScoreArgs a) {
     constexpr int kVec = Piece<T>::kVec;
-    constexpr int N = kBatch * kVec;
+    extern __shared__ uint4 dyn[];       // the ring
     __shared__ ScoreShared sh;
     cg::cluster_group cluster = cg::this_cluster();
     const int parts = static_cast<int>(cluster.num_blocks());
     const int part = static_cast<int>(cluster.block_rank());
-    const int64_t r = blockIdx.x / parts;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int V = static_cast<int>(a.V);
+    const bool top = a.top > 0;
+    const uint32_t step = gridDim.x / static_cast<unsigned>(parts);
+    uint32_t r = blockIdx.x / static_cast<unsigned>(parts);
+    Ring<T> ring(dyn, sh.bars, kStages, &sh.feed, a.logits, a.rows, V, part, parts, nullptr, r, step, a.count, &g_vocab_status);
 
+    auto token_of = [&](uint32_t row) { return a.tokens == nullptr || row >= a.count ? int64_t(-1) : a.tokens[a.tokens_at.at(row)]; };
+    int64_t wanted = token_of(r);
+    T zt = Piece<T>::nan();
+    if (wanted >= 0 && wanted < V) zt = (static_cast<const T*>(a.logits) + a.rows.at(r))[wanted];
+    typename Ring<T>::Place place{0, 0};
+    for (; r < a.count; r += step) {
     const T* row = static_cast<const T*>(a.logits) + a.rows.at(r);
-    const Span<T> span(row, a.V, part, parts);
-    const int64_t token = a.tokens == nullptr ? -1 : a.tokens[a.tokens_at.at(r)];
-    const bool scored = token >= 0 && token < a.V;
-    const float zt = scored ? Piece<T>::one(row[token]) : CUDART_INF_F;
-
-    Stats st{-CUDART_INF_F, 0.0f, 0.0f};
-    int ahead = 0;
-    for (int64_t v = span.first + tid; v < span.last; v += kBatch * kThreads) {
-        float z[N];
-        if (v >= span.lo && v + (kBatch - 1) * kThreads < min(span.hi, span.last)) {
-            uint4 u[kBatch];
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) u[b] = span.grid[v + b * kThreads];
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) Piece<T>::unpack(u[b], z + b * kVec);
-        } else {
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                const int64_t p = v + b * kThreads;
-                if (p < span.last) {
-                    span.load(p, z + b * kVec);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < kVec; ++e) z[b * kVec + e] = -CUDART_INF_F;
-                }
-            }
-        }
-        vocab::take<N, true>(st, z, vocab::kLog2e);
-        if (scored) {
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                if (v + b * kThreads >= span.last) break;
-                const int64_t e0 = span.element(v + b * kThreads);
-                if (e0 > token || e0 + kVec <= token) {
-                    // what lies before the token also counts where it is equal; -inf beyond the row's ends is below or, for a
-                    // token at -inf, has to be left out
-                    const bool before = e0 < token;
-#pragma unroll
-                    for (int e = 0; e < kVec; ++e) {
-                        const float x = z[b * kVec + e];
-                        ahead += x > zt || (before && x == zt && e0 + e >= 0);
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < kVec; ++e) {
-                        const float x = z[b * kVec + e];
-                        ahead += x > zt || (x == zt && e0 + e < token && e0 + e >= 0);
-                    }
-                }
-            }
+    const Span<T> span(row, V, part, parts);
+    const bool scored = wanted >= 0 && wanted < V;
+    const int token = scored ? static_cast<int>(wanted) : -1;
+    const int64_t wanted_next = token_of(r + step);
+    // What is ahead of the token: values >= its own in pieces before its own, values >= the type's next larger one from there on,
+    // and what equals it in front of it in its own piece, which is counted apart.
+    ScoreThread<T> me;
+    me.ahead = 0;
+    me.token_piece = (token + span.shift) / kVec;
+    me.at = me.behind = Piece<T>::word(Piece<T>::nan());
+    if (scored) {
+        me.at = Piece<T>::word(zt);
+        me.behind = Piece<T>::word(Piece<T>::next_up(zt));
+        if (tid < kVec && me.token_piece >= span.first && me.token_piece < span.last) {
+            const int i = span.element(me.token_piece) + tid;
+            if (i >= 0 && i < token) me.ahead += Piece<T>::one(row[i]) == Piece<T>::one(zt);
         }
     }
 
+    const int mine = max(span.end() - span.begin(), 0);
+    const int k = min(a.top, mine);
+    const int pieces = span.whole_last() - span.whole_first();
+    // warps whose lanes all have a piece from the start vote; fewer than four of them: less than kCandidates entries in all, or few rounds
+    const int voters = max(1, min(kWarps, pieces / 32)), j = max(1, (k + voters - 1) / voters), t = (k + j - 1) / j;
+    if (tid == 0) {
+        sh.found = 0;
+        sh.agreed_bound = 0;
+    }
+    me.set_bound(0);
+    __syncthreads();       // the ring's barriers, the count, and nobody is at the row before
+    int round = 0;
+    auto agree = [&]() {       // a bound from what has been read so far
+        if ((round & (round + 1)) == 0) {
+            const uint32_t own = warp_bound(Piece<T>::place(me.run.m), j);
+            if (lane == 0) sh.bound[warp] = own;
+            if (round == 0) __syncthreads();
+            const uint32_t all = sh.agreed(voters, t);
+            if (lane == 0) atomicMax(&sh.agreed_bound, all);
+            __syncwarp();
+        }
+        me.set_bound(*static_cast<volatile uint32_t*>(&sh.agreed_bound));
+        ++round;
+    };
+    for (int i = 0; i < pieces; i += kChunk) {
+        const uint4* chunk = ring.arrive(place);
+        const int v = span.whole_first() + i + tid;
+        if (i + kChunk <= pieces) {
+            uint4 u[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) u[b] = chunk[tid + b * kThreads];
+            const float largest = me.take(u, v);
+            if (top) {
+                agree();
+                me.keep(sh, span, u, v, largest, reinterpret_cast<const T*>(chunk + tid));
+            }
+        } else {
+            // the part's last pieces
+            for (int b = 0; i + b * kThreads < pieces; ++b) {
+                const bool in = i + b * kThreads + tid < pieces;
+                uint4 u[1];
+                float largest = -CUDART_INF_F;
+                if (in) {
+                    u[0] = chunk[tid + b * kThreads];
+                    largest = me.take(u, v + b * kThreads);
+                }
+                if (top) {
+                    __syncwarp();
+                    if (round == 0) agree();
+                    if (in) me.keep(sh, span, u, v + b * kThreads, largest, reinterpret_cast<const T*>(chunk + tid + b * kThreads));
+                }
+            }
+        }
+        ring.release(place);
+        ring.advance(place);
+    }
+    T zt_next = Piece<T>::nan();
+    if (wanted_next >= 0 && wanted_next < V) zt_next = (static_cast<const T*>(a.logits) + a.rows.at(r + step))[wanted_next];
+    // the row's ends; -inf in the places that are not the row's, which a token at -inf would count on the left
+    if ((tid == 0 && span.has_left()) || (tid == 32 && span.has_right())) {
+        const int v = tid == 0 ? span.first : span.last - 1;
+        const uint4 u[1] = {span.load_edge(v)};
+        const float largest = me.take(u, v);
+        if (span.element(v) < 0 && v < me.token_piece && Piece<T>::one(zt) == -CUDART_INF_F) me.ahead += span.element(v);
+        if (top) me.keep(sh, span, u, v, largest, row + span.element(v));
+    }
+
     // the block's statistics
-    const float own_max = st.m;
-    Stats all = vocab::warp_merge(st, vocab::kLog2e);
-    ahead = __reduce_add_sync(0xFFFFFFFFu, ahead);
+    __syncwarp();
+    Stats all = vocab::warp_merge(me.run.stats(vocab::kLog2e), vocab::kLog2e);
+    const int ahead = __reduce_add_sync(0xFFFFFFFFu, me.ahead);
     if (lane == 0) {
         sh.warp[warp] = all;
         sh.warp_ahead[warp] = ahead;
     }
-    if (tid == 0) sh.found = 0;
     __syncthreads();
     if (warp == 0) {
         all = lane < kWarps ? sh.warp[lane] : Stats{-CUDART_INF_F, 0.0f, 0.0f};
@@ -209,76 +352,83 @@ __global__ void __launch_bounds__(kThreads) score_kernel(const ScoreArgs a) {
     }
 
     if (a.top > 0) {
-        const int64_t mine = span.end() - span.begin();
-        const int k = static_cast<int>(min(static_cast<int64_t>(a.top), mine > 0 ? mine : 0));
-        // pieces without a thread of their own never raise a maximum: such threads do not vote
-        const bool has = span.first + tid < span.last;
-        const uint32_t key = vocab::ordered(own_max);
-        uint32_t bound = 0;
-        for (int bit = 31; bit >= 16; --bit) {
-            const uint32_t tryit = bound | (1u << bit);
-            if (__syncthreads_count(has && key >= tryit) >= k) bound = tryit;
-        }
-        if (has && (key >= bound)) {
-            for (int64_t v = span.first + tid; v < span.last; v += kThreads) {
-                float z[kVec];
-                span.load(v, z);
-                const int64_t e0 = span.element(v);
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) {
-                    if (vocab::ordered(z[e]) >= bound && e0 + e >= 0 && e0 + e < a.V) {
-                        const int place = atomicAdd(&sh.found, 1);
-                        if (place < kCandidates) sh.cand[place] = sort_key(z[e], e0 + e);
-                    }
-                }
-            }
-        }
-        __syncthreads();
         int n = sh.found;
-        __syncthreads();
+        me.set_bound(sh.agreed_bound);
+        unsigned long long least = static_cast<unsigned long long>(vocab::ordered(me.bound)) << 32;
         if (n > kCandidates) {
+            __syncthreads();      // everybody has read how many there were
             select_by_radix<T>(sh, row, span.begin(), span.end(), k);
             n = k;
+            least = 0;
+        } else if (n < k) {
+            // fewer entries than that are above -inf, and all of them are kept
+            __syncthreads();
+            take_equal<T>(sh, row, span.begin(), span.end(), vocab::ordered(-CUDART_INF_F), n, k - n);
+            n = k;
+            least = 0;
+        }
+        if (n > kSorted) {
+            // those that the last bound leaves, in their buffer's front
+            unsigned long long mine_of[kCandidates / kThreads];
+#pragma unroll
+            for (int q = 0; q < kCandidates / kThreads; ++q) mine_of[q] = tid + q * kThreads < n ? sh.cand[tid + q * kThreads] : 0ull;
+            __syncthreads();
+            if (tid == 0) sh.found = 0;
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < kCandidates / kThreads; ++q)
+                if (tid + q * kThreads < n && mine_of[q] >= least) sh.cand[atomicAdd(&sh.found, 1)] = mine_of[q];
+            __syncthreads();
+            n = sh.found;
         }
         for (int i = tid; i < n; i += kThreads) {
-            const unsigned long long own = sh.cand[i];
+            const unsigned long long key = sh.cand[i];
             int place = 0;
-            for (int j = 0; j < n; ++j) place += sh.cand[j] > own;
-            if (place < k) sh.best[place] = own;
+            for (int q = 0; q < n; ++q) place += sh.cand[q] > key;
+            if (place < k) sh.best[place] = key;
         }
         if (tid == 0) sh.listed = k;
     }
-    cluster.sync();
+    if (parts > 1) cluster.sync();
+    else __syncthreads();
 
     if (part == 0) {
-        Stats total = sh.mine;
-        int before = sh.ahead;
-        for (int p = 1; p < parts; ++p) {
-            const ScoreShared* other = cluster.map_shared_rank(&sh, p);
-            total = vocab::merge(total, other->mine, vocab::kLog2e);
-            before += other->ahead;
+        if (parts > 1) {
+            // the others' statistics, a lane each, and lists, all at once
+            if (warp == 0) {
+                const ScoreShared* other = cluster.map_shared_rank(&sh, min(lane, parts - 1));
+                const Stats total = vocab::warp_merge(lane < parts ? other->mine : Stats{-CUDART_INF_F, 0.0f, 0.0f}, vocab::kLog2e);
+                const int before = __reduce_add_sync(0xFFFFFFFFu, lane < parts ? other->ahead : 0);
+                if (lane < parts) sh.lengths[lane] = other->listed;
+                __syncwarp();
+                if (lane == 0) {
+                    sh.mine = total;
+                    sh.ahead = before;
+                }
+            }
+            for (int i = tid; i < parts * a.top; i += kThreads) sh.cand[i] = cluster.map_shared_rank(&sh, i / a.top)->best[i % a.top];
+            __syncthreads();
         }
+        const Stats total = sh.mine;
         const float log_s = logf(total.s);
         if (tid == 0) {
-            if (a.logprobs != nullptr) a.logprobs[r] = scored ? (zt - total.m) - log_s : 0.0f;
-            if (a.ranks != nullptr) a.ranks[r] = scored ? before : -1;
+            if (a.logprobs != nullptr) a.logprobs[r] = scored ? (Piece<T>::one(zt) - total.m) - log_s : 0.0f;
+            if (a.ranks != nullptr) a.ranks[r] = scored ? sh.ahead : -1;
             // entropy = lse - sum p z = log s - (sum e d) ln 2 / s with d = log2 e; a row of -inf has none
             if (a.entropy != nullptr) a.entropy[r] = total.m == -CUDART_INF_F ? CUDART_NAN_F : log_s - total.w * vocab::kLn2 / total.s;
         }
         // every CTA's list is in order: an entry's place is its own plus, in each other list, how many come before it
         for (int i = tid; i < parts * a.top; i += kThreads) {
             const int p = i / a.top, q = i % a.top;
-            const ScoreShared* list = cluster.map_shared_rank(&sh, p);
-            if (q >= list->listed) continue;
-            const unsigned long long key = list->best[q];
+            if (q >= (parts > 1 ? sh.lengths[p] : sh.listed)) continue;
+            const unsigned long long key = parts > 1 ? sh.cand[i] : sh.best[q];
             int place = q;
             for (int o = 0; o < parts; ++o) {
                 if (o == p) continue;
-                const ScoreShared* other = cluster.map_shared_rank(&sh, o);
-                int lo = 0, hi = other->listed;
+                int lo = 0, hi = sh.lengths[o];
                 while (lo < hi) {
                     const int mid = (lo + hi) >> 1;
-                    if (other->best[mid] > key) lo = mid + 1;
+                    if (sh.cand[o * a.top + mid] > key) lo = mid + 1;
                     else hi = mid;
                 }
                 place += lo;
@@ -290,25 +440,45 @@ __global__ void __launch_bounds__(kThreads) score_kernel(const ScoreArgs a) {
             }
         }
     }
-    cluster.sync();      // CTA 0 reads the others' shared memory
+    if (parts > 1) cluster.sync();      // CTA 0 reads the others' shared memory
+    else __syncthreads();
+    wanted = wanted_next;
+    zt = zt_next;
+    }
 }
 
-// CTAs per row: as many as fill the GPU once with two CTAs per SM, each with at least two batches of the threads' pieces.
-int parts_for(int64_t rows, int64_t V, int esz) {
-    const int64_t pieces = (V * esz + 15) / 16;
-    int parts = 1;
-    while (parts < vocab::kMaxCluster && rows * parts * 2 <= 2 * static_cast<int64_t>(sm_count()) && pieces >= static_cast<int64_t>(parts) * 2 * kThreads * 2) parts *= 2;
-    return parts;
+// CTAs per row and rows under way. As many CTAs as the GPU holds walk over the rows; a CTA's time for a row is about its bytes at 11 per
+// ns (a quarter of an SM's share of the memory's rate) and 3 us for what the row's end takes, which the other CTAs of the SM fill. The
+// number of parts for which the longest walk is shortest.
+constexpr double kSmRate = 42000.0;     // bytes per us of an SM's share of the memory's rate
+constexpr double kEnd = 6.0;            // us of a row's end, by which parts cost
+struct Walk {
+    int parts;
+    int64_t clusters;
+};
+Walk walk_over(int64_t rows, int64_t V, int esz, int least_parts, int per_sm) {
+    const int64_t slots = static_cast<int64_t>(per_sm) * sm_count();
+    Walk best{0, 0};
+    double least = 0.0;
+    for (int parts = least_parts; parts <= vocab::kMaxCluster; parts *= 2) {
+        const int64_t clusters = std::min(rows, std::max<int64_t>(1, slots / parts));
+        const double cost = static_cast<double>((rows + clusters - 1) / clusters) * (static_cast<double>(V) * esz / parts * per_sm / kSmRate + kEnd);
+        if (best.parts == 0 || cost < least) {
+            least = cost;
+            best = Walk{parts, clusters};
+        }
+    }
+    return best;
 }
 
 template <typename Kernel, typename... Args>
-int launch_rows(Kernel kernel, int64_t rows, int parts, int64_t smem, cudaStream_t stream, const char* what, const Args&... args) {
+int launch_rows(Kernel kernel, const Walk& walk, int64_t smem, cudaStream_t stream, const char* what, const Args&... args) {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(parts);
+    attr[0].val.clusterDim.x = static_cast<unsigned>(walk.parts);
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(rows * parts), 1, 1);
+    cfg.gridDim = dim3(static_cast<unsigned>(walk.clusters * walk.parts), 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
     cfg.dynamicSmemBytes = static_cast<size_t>(smem);
     cfg.stream = stream;
@@ -320,6 +490,26 @@ int launch_rows(Kernel kernel, int64_t rows, int parts, int64_t smem, cudaStream
         return BSI_ERR_CUDA;
     }
     return BSI_OK;
+}
+
+constexpr int kRingBytes = kStages * kChunk * 16;
+
+template <typename Kernel>
+int allow_shared(Kernel kernel, int bytes, bool (&set)[64]) {
+    int dev = 0;
+    BSI_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !set[dev]) {
+        BSI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        if (dev >= 0 && dev < 64) set[dev] = true;
+    }
+    return BSI_OK;
+}
+
+template <typename T>
+int launch_score(const ScoreArgs& a, int64_t rows, cudaStream_t stream) {
+    static bool set[64] = {false};
+    if (int rc = allow_shared(score_kernel<T>, kRingBytes, set)) return rc;
+    return launch_rows(score_kernel<T>, walk_over(rows, a.V, sizeof(T), 1, kPerSm), kRingBytes, stream, "token_logprobs", a);
 }
 
 constexpr int64_t kMaxRows = 0x7FFFFFFFll / vocab::kMaxCluster;
@@ -363,6 +553,7 @@ RowPlan plan_of(const bsi_row_plan* p) { return RowPlan{p->per, p->block_stride,
 struct DistillArgs {
     const void* logits;
     RowPlan rows;
+    uint32_t count;              // rows
     int64_t V;
     const int64_t* ids;          // [rows, K]
     const void* teacher;         // [rows, K]
@@ -389,8 +580,9 @@ struct Entry {
 };
 
 struct DistillShared {
-    Stats warp[kWarps];
+    Stats warp[kWarps], warp_listed[kWarps];
     float part[kWarps];
+    vocab::Feed feed;
     Stats rest, listed;          // of this CTA's part of the row, read by the other CTAs
     float total_p;
     Entry entry[kMaxListed];
@@ -402,7 +594,7 @@ __device__ __forceinline__ float teacher_value(const void* t, int dtype, int64_t
     return __bfloat162float(static_cast<const __nv_bfloat16*>(t)[i]);
 }
 
-// The row's entries with their probabilities and logits, by warp 0 alone (a few values per lane); the caller synchronises.
+// The row's entries with their probabilities and logits, by one warp (a few values per lane); the caller synchronises.
 template <typename T>
 __device__ void read_entries(DistillShared& sh, const DistillArgs& a, int64_t r, const T* row) {
     const int lane = threadIdx.x & 31;
@@ -472,62 +664,76 @@ __device__ __forceinline__ bool first_of_id(const DistillShared& sh, int K, int 
     return first;
 }
 
-// The gradient of the pieces [first, last) of a row: factor * q_j everywhere, then the listed logits by themselves.
-// cached: the pieces as they were read by this CTA, or null to read them again.
+// The gradient of a part of a row: factor * q_j everywhere, then the listed logits by themselves.
 template <typename T>
-__device__ void write_grad(DistillShared& sh, const DistillArgs& a, int64_t r, const Span<T>& span, const uint4* cached, float4 saved,
-                           float scale) {
-    constexpr int kVec = Piece<T>::kVec;
-    T* out = static_cast<T*>(a.grad) + r * a.grad_stride;
-    const float c = vocab::kLog2e / a.temperature;
-    const float rest = scale * saved.z * saved.y, top = scale * saved.y;
-    const bool vector = (reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(T) == static_cast<unsigned>(span.shift);
-    uint4* out_grid = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(out) & ~uintptr_t(15));
-    const bool on = saved.w != 0.0f && scale != 0.0f;
-    for (int64_t v0 = span.first + threadIdx.x; v0 < span.last; v0 += kBatch * kThreads) {
-        uint4 u[kBatch];
+struct Gradient {
+    static constexpr int kVec = Piece<T>::kVec;
+    T* out;
+    uint4* out_grid;
+    float c, m, rest, top, scale;
+    bool vector, on;
+
+    __device__ __forceinline__ Gradient(const DistillArgs& a, uint32_t r, const Span<T>& span, const float4& saved, float s)
+        : out(static_cast<T*>(a.grad) + r * a.grad_stride), c(vocab::kLog2e / a.temperature), m(saved.x), rest(s * saved.z * saved.y), top(s * saved.y),
+          scale(s), vector((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(T) == static_cast<unsigned>(span.shift)), on(saved.w != 0.0f && s != 0.0f) {
+        out_grid = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(out) & ~uintptr_t(15));
+    }
+    __device__ __forceinline__ void write(const Span<T>& span, const uint4& u, int v) const {
+        float z[kVec];
         if (on) {
+            Piece<T>::unpack(u, z);
+            const vocab::Two less(-m, -m), cc(c, c), rr(rest, rest);
 #pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                const int64_t v = v0 + b * kThreads;
-                if (v < span.last && (cached != nullptr || span.whole(v))) u[b] = cached != nullptr ? cached[v - span.first] : span.grid[v];
+            for (int e = 0; e < kVec; e += 2) {
+                float d0, d1;
+                vocab::mul2(vocab::add2(vocab::Two(z[e], z[e + 1]), less), cc).split(d0, d1);
+                vocab::mul2(vocab::Two(vocab::exp2_fast(d0), vocab::exp2_fast(d1)), rr).split(z[e], z[e + 1]);
             }
+        } else {
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) z[e] = 0.0f;
         }
+        if (vector && span.whole(v)) {
+            out_grid[v] = Piece<T>::pack(z);
+        } else {
+            const int e0 = span.element(v);
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            const int64_t v = v0 + b * kThreads;
-            if (v >= span.last) break;
-            float z[kVec], g[kVec];
-            if (on) {
-                if (cached != nullptr || span.whole(v)) Piece<T>::unpack(u[b], z);
-                else span.load_edge(v, z);
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) g[e] = rest * vocab::exp2_fast((z[e] - saved.x) * c);
-            } else {
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) g[e] = 0.0f;
-            }
-            if (vector && span.whole(v)) {
-                out_grid[v] = Piece<T>::pack(g);
-            } else {
-                const int64_t e0 = span.element(v);
-#pragma unroll
-                for (int e = 0; e < kVec; ++e)
-                    if (e0 + e >= 0 && e0 + e < a.V) out[e0 + e] = Piece<T>::narrow(g[e]);
-            }
+            for (int e = 0; e < kVec; ++e)
+                if (e0 + e >= 0 && e0 + e < span.V) out[e0 + e] = Piece<T>::narrow(z[e]);
         }
     }
-    if (!on) return;
-    __syncthreads();       // the pieces are written before the listed logits' own values
-    const int64_t lo = span.begin(), hi = span.end();
-    for (int k = threadIdx.x; k < a.K; k += kThreads) {
-        const int id = sh.entry[k].id;
-        if (id < lo || id >= hi) continue;
-        float p;
-        if (!first_of_id(sh, a.K, k, &p)) continue;
-        out[id] = Piece<T>::narrow(top * vocab::exp2_fast((sh.entry[k].z - saved.x) * c) - scale * p);
+    // From memory.
+    __device__ __forceinline__ void write_part(const Span<T>& span) const {
+        const int last = span.whole_last();
+        int v = span.whole_first() + threadIdx.x;
+        const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+        for (; v + (kBatch - 1) * kThreads < last; v += kChunk) {
+            uint4 u[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) u[b] = on ? span.grid[v + b * kThreads] : none;
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) write(span, u[b], v + b * kThreads);
+        }
+        for (; v < last; v += kThreads) write(span, on ? span.grid[v] : none, v);
     }
-}
+    __device__ __forceinline__ void write_ends(const Span<T>& span) const {
+        if ((threadIdx.x == 0 && span.has_left()) || (threadIdx.x == 32 && span.has_right())) {
+            const int v = threadIdx.x == 0 ? span.first : span.last - 1;
+            write(span, span.load_edge(v), v);
+        }
+    }
+    // Behind a barrier of the block: the pieces are written, and the entries have been read.
+    __device__ __forceinline__ void write_listed(const DistillShared& sh, const Span<T>& span, int K) const {
+        const int lo = span.begin(), hi = span.end();
+        for (int k = threadIdx.x; k < K; k += kThreads) {
+            const int id = sh.entry[k].id;
+            if (id < lo || id >= hi) continue;
+            float p;
+            if (!first_of_id(sh, K, k, &p)) continue;
+            out[id] = Piece<T>::narrow(top * vocab::exp2_fast((sh.entry[k].z - m) * c) - scale * p);
+        }
+    }
+};
 
 __device__ __forceinline__ float grad_scale(const DistillArgs& a, int64_t r) {
     const float w = a.weights != nullptr ? a.weights[r] : 1.0f;
@@ -537,130 +743,148 @@ __device__ __forceinline__ float grad_scale(const DistillArgs& a, int64_t r) {
     return up * a.temperature * (w / d);
 }
 
-// The forward pass; GRAD: the gradient too, from the row's pieces that the cluster keeps in shared memory.
-// Dynamic shared memory: with the tail on, one bit per logit of the part; with GRAD, the part's pieces.
+// The forward pass; GRAD: the gradient too, while L2 still holds the row. Dynamic shared memory: with the tail on, one bit per logit of
+// the part; the ring.
 template <typename T, bool GRAD>
-__global__ void __launch_bounds__(kThreads) distill_kernel(const DistillArgs a, int bit_words) {
+__global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const DistillArgs a, int bit_words, int stages) {
     constexpr int kVec = Piece<T>::kVec;
-    constexpr int N = kBatch * kVec;
     extern __shared__ uint4 dyn[];
     __shared__ DistillShared sh;
     uint32_t* bits = reinterpret_cast<uint32_t*>(dyn);
-    uint4* cache = dyn + bit_words / 4;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(dyn + bit_words / 4);
+    uint4* data = dyn + bit_words / 4 + stages;      // two barriers a stage
     cg::cluster_group cluster = cg::this_cluster();
     const int parts = static_cast<int>(cluster.num_blocks());
     const int part = static_cast<int>(cluster.block_rank());
-    const int64_t r = blockIdx.x / parts;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int V = static_cast<int>(a.V);
+    const uint32_t step = gridDim.x / static_cast<unsigned>(parts);
+    uint32_t r = blockIdx.x / static_cast<unsigned>(parts);
+    Ring<T> ring(data, bars, stages, &sh.feed, a.logits, a.rows, V, part, parts, a.weights, r, step, a.count, &g_vocab_status);
+    typename Ring<T>::Place place{0, 0};
+    for (; r < a.count; r += step) {
     const T* row = static_cast<const T*>(a.logits) + a.rows.at(r);
-    const Span<T> span(row, a.V, part, parts);
+    const Span<T> span(row, V, part, parts);
 
     if (a.weights != nullptr && a.weights[r] == 0.0f) {      // every CTA of the cluster alike: a padded row is not read
         if (part == 0 && tid == 0) {
             a.row_loss[r] = 0.0f;
             if (a.saved != nullptr) a.saved[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
-        if (GRAD) write_grad<T>(sh, a, r, span, nullptr, make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f);
-        return;
+        if (GRAD) {
+            const Gradient<T> g(a, r, span, make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f);
+            g.write_part(span);
+            g.write_ends(span);
+        }
+        continue;
     }
+    __syncthreads();      // nobody is at the row before
 
-    if (warp == 0) read_entries<T>(sh, a, r, row);
+    // The last warp reads the entries; with the tail off nobody waits for it before the row's end
+    if (warp == kWarps - 1) read_entries<T>(sh, a, r, row);
+    const float c = vocab::kLog2e / a.temperature;
+    const int bit0 = span.element(span.first);         // the part's bit 0; kVec bits for each piece
+    const int lo = span.begin(), hi = span.end();
     if (a.tail) {
         for (int i = tid; i < bit_words; i += kThreads) bits[i] = 0u;
-    }
-    __syncthreads();
-    const float c = vocab::kLog2e / a.temperature;
-    const int64_t bit0 = span.first * kVec - span.shift;         // the part's bit 0; kVec bits for each piece
-    if (a.tail) {
+        __syncthreads();
         for (int k = tid; k < a.K; k += kThreads) {
-            const int64_t id = sh.entry[k].id;
-            if (id >= span.begin() && id < span.end()) atomicOr(&bits[(id - bit0) >> 5], 1u << ((id - bit0) & 31));
+            const int id = sh.entry[k].id;
+            if (id >= lo && id < hi) atomicOr(&bits[(id - bit0) >> 5], 1u << ((id - bit0) & 31));
         }
         __syncthreads();
     }
 
-    Stats st{-CUDART_INF_F, 0.0f, 0.0f};
-    for (int64_t v = span.first + tid; v < span.last; v += kBatch * kThreads) {
-        float z[N];
-        if (v >= span.lo && v + (kBatch - 1) * kThreads < min(span.hi, span.last)) {
+    vocab::Running<T, false> run;
+    __syncthreads();
+    // a piece as the statistics see it: listed logits out where they are summed apart
+    auto seen = [&](uint4& u, int v) {
+        if (a.tail) {
+            const int p = (v - span.first) * kVec;
+            const uint32_t mask = (bits[p >> 5] >> (p & 31)) & ((1u << kVec) - 1u);
+            if (mask != 0u) {
+                float z[kVec];
+                Piece<T>::unpack(u, z);
+#pragma unroll
+                for (int e = 0; e < kVec; ++e)
+                    if ((mask >> e) & 1u) z[e] = -CUDART_INF_F;
+                u = Piece<T>::pack(z);
+            }
+        }
+    };
+    const int pieces = span.whole_last() - span.whole_first();
+    for (int i = 0; i < pieces; i += kChunk) {
+        const uint4* chunk = ring.arrive(place);
+        const int v = span.whole_first() + i + tid;
+        if (i + kChunk <= pieces) {
             uint4 u[kBatch];
 #pragma unroll
-            for (int b = 0; b < kBatch; ++b) u[b] = span.grid[v + b * kThreads];
+            for (int b = 0; b < kBatch; ++b) u[b] = chunk[tid + b * kThreads];
+            ring.release(place);
 #pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                Piece<T>::unpack(u[b], z + b * kVec);
-                if (GRAD) cache[v + b * kThreads - span.first] = u[b];
-            }
+            for (int b = 0; b < kBatch; ++b) seen(u[b], v + b * kThreads);
+            run.take(u, c);
         } else {
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                const int64_t p = v + b * kThreads;
-                if (p < span.last) {
-                    span.load(p, z + b * kVec);
-                    if (GRAD) cache[p - span.first] = Piece<T>::pack(z + b * kVec);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < kVec; ++e) z[b * kVec + e] = -CUDART_INF_F;
-                }
+            for (int b = 0; i + b * kThreads + tid < pieces; ++b) {
+                uint4 u[1] = {chunk[tid + b * kThreads]};
+                seen(u[0], v + b * kThreads);
+                run.take(u, c);
             }
+            ring.release(place);
         }
-        if (a.tail) {
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                const int64_t p = v + b * kThreads - span.first;
-                if (p >= span.last - span.first) break;
-                const uint32_t mask = (bits[p * kVec >> 5] >> ((p * kVec) & 31)) & ((1u << kVec) - 1u);
-                if (mask != 0u) {
-#pragma unroll
-                    for (int e = 0; e < kVec; ++e)
-                        if ((mask >> e) & 1u) z[b * kVec + e] = -CUDART_INF_F;
-                }
-            }
-        }
-        vocab::take<N, false>(st, z, c);
+        ring.advance(place);
     }
+    if ((tid == 0 && span.has_left()) || (tid == 32 && span.has_right())) {
+        const int v = tid == 0 ? span.first : span.last - 1;
+        uint4 u[1] = {span.load_edge(v)};
+        seen(u[0], v);
+        run.take(u, c);
+    }
+    __syncwarp();
 
+    Stats st = vocab::warp_merge(run.stats(c), c);
+    if (lane == 0) sh.warp[warp] = st;
+    __syncthreads();
     Stats listed{-CUDART_INF_F, 0.0f, 0.0f};
     if (a.tail) {
         for (int k = tid; k < a.K; k += kThreads) {
-            const int64_t id = sh.entry[k].id;
+            const int id = sh.entry[k].id;
             float p;
-            if (id >= span.begin() && id < span.end() && first_of_id(sh, a.K, k, &p)) {
-                const float z[1] = {sh.entry[k].z};
-                vocab::take<1, false>(listed, z, c);
-            }
+            if (id >= lo && id < hi && first_of_id(sh, a.K, k, &p)) listed = vocab::merge(listed, Stats{sh.entry[k].z, sh.entry[k].z == -CUDART_INF_F ? 0.0f : 1.0f, 0.0f}, c);
         }
-    }
-    st = vocab::warp_merge(st, c);
-    if (lane == 0) sh.warp[warp] = st;
-    __syncthreads();
-    if (warp == 0) {
-        st = vocab::warp_merge(lane < kWarps ? sh.warp[lane] : Stats{-CUDART_INF_F, 0.0f, 0.0f}, c);
-        if (lane == 0) sh.rest = st;
-    }
-    if (a.tail) {
         listed = vocab::warp_merge(listed, c);
+        if (lane == 0) sh.warp_listed[warp] = listed;
         __syncthreads();
-        if (lane == 0) sh.warp[warp] = listed;
-        __syncthreads();
-        if (warp == 0) {
-            listed = vocab::warp_merge(lane < kWarps ? sh.warp[lane] : Stats{-CUDART_INF_F, 0.0f, 0.0f}, c);
-            if (lane == 0) sh.listed = listed;
+    }
+    if (warp == 0) {
+        const Stats none{-CUDART_INF_F, 0.0f, 0.0f};
+        st = vocab::warp_merge(lane < kWarps ? sh.warp[lane] : none, c);
+        if (a.tail) listed = vocab::warp_merge(lane < kWarps ? sh.warp_listed[lane] : none, c);
+        if (lane == 0) {
+            sh.rest = st;
+            sh.listed = listed;
         }
-    } else if (tid == 0) {
-        sh.listed = Stats{-CUDART_INF_F, 0.0f, 0.0f};
     }
-    cluster.sync();
+    if (parts > 1) cluster.sync();
+    else __syncthreads();
 
-    // every CTA joins the parts in the same order
-    Stats rest = cluster.map_shared_rank(&sh, 0)->rest, all = cluster.map_shared_rank(&sh, 0)->listed;
-    for (int p = 1; p < parts; ++p) {
-        const DistillShared* other = cluster.map_shared_rank(&sh, p);
-        rest = vocab::merge(rest, other->rest, c);
-        all = vocab::merge(all, other->listed, c);
+    // every CTA joins the parts in the same way, a lane for each
+    if (parts > 1) {
+        if (warp == 0) {
+            const Stats none{-CUDART_INF_F, 0.0f, 0.0f};
+            const DistillShared* other = cluster.map_shared_rank(&sh, min(lane, parts - 1));
+            st = vocab::warp_merge(lane < parts ? other->rest : none, c);
+            listed = vocab::warp_merge(lane < parts ? other->listed : none, c);
+        }
+        cluster.sync();      // nobody's shared memory is read by another after this
+        if (tid == 0) {
+            sh.rest = st;
+            sh.listed = listed;
+        }
+        __syncthreads();
     }
-    all = vocab::merge(rest, all, c);
-    cluster.sync();      // nobody's shared memory is read after this
+    const Stats rest = sh.rest;
+    const Stats all = a.tail ? vocab::merge(rest, sh.listed, c) : rest;
 
     // Rows of at most K logits may be listed whole: then there is no rest, whatever rounding leaves of the teacher's sum.
     bool outside = true;
@@ -693,21 +917,30 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(const DistillArgs a, 
             if (a.saved != nullptr) a.saved[r] = saved;
         }
     }
-    if (GRAD) write_grad<T>(sh, a, r, span, cache, saved, grad_scale(a, r));
+    if (GRAD) {
+        // the row again, out of L2: what the resident CTAs are at is a third of it
+        const Gradient<T> g(a, r, span, saved, grad_scale(a, r));
+        g.write_part(span);
+        g.write_ends(span);
+        __syncthreads();
+        if (g.on) g.write_listed(sh, span, a.K);
+    }
+    }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_backward_kernel(const DistillArgs a, int parts) {
+__global__ void __launch_bounds__(kThreads, 4) distill_backward_kernel(const DistillArgs a, int parts) {
     __shared__ DistillShared sh;
-    const int64_t r = blockIdx.x / parts;
+    const uint32_t r = blockIdx.x / static_cast<unsigned>(parts);
     const T* row = static_cast<const T*>(a.logits) + a.rows.at(r);
-    const Span<T> span(row, a.V, static_cast<int>(blockIdx.x % parts), parts);
+    const Span<T> span(row, static_cast<int>(a.V), static_cast<int>(blockIdx.x % parts), parts);
     const float4 saved = a.saved[r];
-    if (saved.w != 0.0f) {
-        if (threadIdx.x < 32) read_entries<T>(sh, a, r, row);
-        __syncthreads();
-    }
-    write_grad<T>(sh, a, r, span, nullptr, saved, grad_scale(a, r));
+    if (saved.w != 0.0f && threadIdx.x >= kThreads - 32) read_entries<T>(sh, a, r, row);
+    const Gradient<T> g(a, r, span, saved, grad_scale(a, r));
+    g.write_part(span);
+    g.write_ends(span);
+    __syncthreads();
+    if (g.on) g.write_listed(sh, span, a.K);
 }
 
 // totals[0] = the rows' losses summed (mean: over the weights' sum), totals[1] = the weights' sum. One block: a fixed order.
@@ -744,37 +977,43 @@ __global__ void __launch_bounds__(kTotalThreads) distill_totals_kernel(const flo
     }
 }
 
-// Shared memory of a part in distill_kernel; the bits first, whole 16-byte pieces.
+// Dynamic shared memory of a part in distill_kernel: bits (in the row's pieces, whatever its offset), two barriers a stage, the stages.
 template <typename T>
-int part_bytes(int64_t V, int parts, bool tail, bool grad, int* bit_words) {
-    const int64_t pieces = (V + 2 * Piece<T>::kVec - 2) / Piece<T>::kVec;      // whatever the row's offset
-    const int64_t mine = (pieces + parts - 1) / parts + 1;
+int64_t part_bytes(int64_t V, int parts, bool tail, int* bit_words) {
+    const int64_t mine = ((V + 2 * Piece<T>::kVec - 2) / Piece<T>::kVec + parts - 1) / parts + 1;
     *bit_words = tail ? static_cast<int>((mine * Piece<T>::kVec + 127) / 128 * 4) : 0;
-    const int64_t bytes = *bit_words * 4ll + (grad ? mine * 16 : 0);
-    return bytes > 0x7FFFFFFF ? 0x7FFFFFFF : static_cast<int>(bytes);
+    return *bit_words * 4ll + kStages * 16ll + kRingBytes;
 }
 
+constexpr int64_t kSmShared = 227 * 1024;
 constexpr int kPartLimit = 200 * 1024;      // dynamic shared memory of a CTA, beside about 10 KB of static
 
 template <typename T, bool GRAD>
 int launch_distill(const DistillArgs& a, int64_t rows, cudaStream_t stream) {
-    static bool attr_set[64] = {false};
-    int dev = 0;
-    BSI_CUDA_TRY(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-        BSI_CUDA_TRY(cudaFuncSetAttribute(distill_kernel<T, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPartLimit));
-        if (dev >= 0 && dev < 64) attr_set[dev] = true;
-    }
-    int parts = parts_for(rows, a.V, sizeof(T)), words = 0;
-    while (parts < vocab::kMaxCluster && part_bytes<T>(a.V, parts, a.tail != 0, GRAD, &words) > kPartLimit) parts *= 2;
-    const int bytes = part_bytes<T>(a.V, parts, a.tail != 0, GRAD, &words);
-    if (bytes > kPartLimit) return fail(BSI_ERR_UNSUPPORTED, "distill: a row of this length does not fit the shared memory of a cluster");
-    return launch_rows(distill_kernel<T, GRAD>, rows, parts, bytes, stream, "distill", a, words);
+    static bool set[64] = {false};
+    if (int rc = allow_shared(distill_kernel<T, GRAD>, kPartLimit, set)) return rc;
+    // a vocabulary whose bits no part holds alone is shared by more
+    int least = 1, words = 0;
+    while (least < vocab::kMaxCluster && part_bytes<T>(a.V, least, a.tail != 0, &words) > kPartLimit) least *= 2;
+    const int64_t largest = part_bytes<T>(a.V, least, a.tail != 0, &words);
+    if (largest > kPartLimit) return fail(BSI_ERR_UNSUPPORTED, "distill: the bits of a vocabulary of this size do not fit a cluster's shared memory");
+    const int per_sm = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kPerSm, kSmShared / (largest + static_cast<int64_t>(sizeof(DistillShared)) + 1024))));
+    const Walk walk = walk_over(rows, a.V, sizeof(T), least, per_sm);
+    const int64_t bytes = part_bytes<T>(a.V, walk.parts, a.tail != 0, &words);
+    return launch_rows(distill_kernel<T, GRAD>, walk, bytes, stream, "distill", a, words, kStages);
+}
+
+// CTAs per row of the backward pass, which has nothing to join: at least two rounds of the GPU's slots, and chunks enough for each.
+int pieces_apart(int64_t rows, int64_t V, int esz) {
+    const int64_t chunks = (V * esz + kChunk * 16 - 1) / (kChunk * 16);
+    int64_t parts = 1;
+    while (parts < 64 && rows * parts < 8ll * sm_count() && chunks >= parts * 2) parts *= 2;
+    return static_cast<int>(parts);
 }
 
 template <typename T>
 int launch_distill_backward(const DistillArgs& a, int64_t rows, cudaStream_t stream) {
-    const int parts = parts_for(rows, a.V, sizeof(T));
+    const int parts = pieces_apart(rows, a.V, sizeof(T));
     distill_backward_kernel<T><<<static_cast<unsigned>(rows * parts), kThreads, 0, stream>>>(a, parts);
     return check_launch("distill_backward launch");
 }
@@ -821,14 +1060,13 @@ extern "C" int bsi_b200_token_logprobs(const void* logits, int dtype, int64_t ro
     if (top > 0 && (top_logprobs == nullptr || top_ids == nullptr)) return fail(BSI_ERR_INVALID, "token_logprobs: null output for the top alternatives");
     rc = require_sm100();
     if (rc != BSI_OK) return rc;
-    ScoreArgs a{logits, plan_of(plan), V, tokens, tokens != nullptr ? plan_of(token_plan) : RowPlan{0, 0, 0}, top,
+    ScoreArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, tokens, tokens != nullptr ? plan_of(token_plan) : RowPlan{0, 0, 0}, top,
                 logprobs, ranks, entropy, top_logprobs, top_ids};
-    const int parts = parts_for(rows, V, dtype == BSI_DTYPE_F32 ? 4 : 2);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (dtype) {
-        case BSI_DTYPE_F32: return launch_rows(score_kernel<float>, rows, parts, 0, s, "token_logprobs", a);
-        case BSI_DTYPE_F16: return launch_rows(score_kernel<__half>, rows, parts, 0, s, "token_logprobs", a);
-        default: return launch_rows(score_kernel<__nv_bfloat16>, rows, parts, 0, s, "token_logprobs", a);
+        case BSI_DTYPE_F32: return launch_score<float>(a, rows, s);
+        case BSI_DTYPE_F16: return launch_score<__half>(a, rows, s);
+        default: return launch_score<__nv_bfloat16>(a, rows, s);
     }
 }
 
@@ -844,7 +1082,7 @@ extern "C" int bsi_b200_distill_forward(const void* logits, int dtype, int64_t r
     rc = require_sm100();
     if (rc != BSI_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    DistillArgs a{logits, plan_of(plan), V, ids, teacher, teacher_dtype, K, temperature, tail != 0, weights, row_loss,
+    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, temperature, tail != 0, weights, row_loss,
                   reinterpret_cast<float4*>(saved), nullptr, 0, nullptr, nullptr, 0};
     if (rows > 0) {
         rc = dtype == BSI_DTYPE_F32 ? launch_distill<float, false>(a, rows, s)
@@ -870,19 +1108,10 @@ extern "C" int bsi_b200_distill_backward(const void* logits, int dtype, int64_t 
     rc = require_sm100();
     if (rc != BSI_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    DistillArgs a{logits, plan_of(plan), V, ids, teacher, teacher_dtype, K, temperature, tail != 0, weights, nullptr,
+    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, temperature, tail != 0, weights, nullptr,
                   const_cast<float4*>(reinterpret_cast<const float4*>(saved)), upstream, upstream_stride, denominator, grad, grad_stride};
     return dtype == BSI_DTYPE_F32 ? launch_distill_backward<float>(a, rows, s)
            : dtype == BSI_DTYPE_F16 ? launch_distill_backward<__half>(a, rows, s) : launch_distill_backward<__nv_bfloat16>(a, rows, s);
-}
-
-extern "C" int bsi_b200_distill_fused_fits(int dtype, int64_t V, int tail) {
-    using namespace bsi;
-    int words = 0;
-    if (V < 1 || V > 0x7FFFFFFFll) return 0;
-    const int bytes = dtype == BSI_DTYPE_F32 ? part_bytes<float>(V, vocab::kMaxCluster, tail != 0, true, &words)
-                                             : part_bytes<__half>(V, vocab::kMaxCluster, tail != 0, true, &words);
-    return bytes <= kPartLimit ? 1 : 0;
 }
 
 extern "C" int bsi_b200_distill_fused(const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan,
@@ -903,7 +1132,7 @@ extern "C" int bsi_b200_distill_fused(const void* logits, int dtype, int64_t row
         rc = check_launch("distill weights launch");
         if (rc != BSI_OK) return rc;
     }
-    DistillArgs a{logits, plan_of(plan), V, ids, teacher, teacher_dtype, K, temperature, tail != 0, weights, row_loss,
+    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, temperature, tail != 0, weights, row_loss,
                   nullptr, nullptr, 0, mean ? weight_sum : nullptr, grad, grad_stride};
     if (rows > 0) {
         rc = dtype == BSI_DTYPE_F32 ? launch_distill<float, true>(a, rows, s)

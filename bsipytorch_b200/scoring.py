@@ -89,7 +89,7 @@ def distillation_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Te
 
 def distillation_loss_and_grad(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, temperature: float = 1.0, tail: bool = False,
                                weights: Optional[torch.Tensor] = None, reduction: str = "mean"):
-    """(distillation_loss(...), its gradient for ``logits``) from one pass: the logits are read once, so a loop that drives its
-    backward pass by hand (``logits.backward(grad)``) moves a third less than through autograd. Needs rows that fit the shared memory
-    of a cluster of CTAs: about 390,000 float32 or 780,000 16-bit logits. ``none``: one loss per row, the gradient of their sum."""
+    """(distillation_loss(...), its gradient for ``logits``) from one pass: the logits come from memory once, so a loop that drives its
+    backward pass by hand (``logits.backward(grad)``) moves a third less than through autograd. ``none``: one loss per row, the gradient
+    of their sum."""
     return _ops().distill_fused(logits, ids, teacher, float(temperature), bool(tail), weights, _reduction(reduction))

@@ -477,9 +477,8 @@ int bsi_b200_distill_backward(const void* logits, int dtype, int64_t rows, int64
                               const int64_t* ids, const void* teacher, int teacher_dtype, int K, float temperature, int tail,
                               const float* weights, const float* saved, const float* upstream, int64_t upstream_stride,
                               const float* denominator, void* grad, int64_t grad_stride, bsi_stream_t stream);
-/* Both at once, the logits read once: a row stays in the shared memory of the CTAs that share it. Same loss, and the gradient of
- * `loss`. For rows that fit (host function, 1 or 0: about 390,000 float32 or 780,000 16-bit logits). loss and weight_sum are needed. */
-int bsi_b200_distill_fused_fits(int dtype, int64_t V, int tail);
+/* Both at once, the logits read from memory once: a row's second reading comes out of L2. Same loss, and the gradient of `loss`. loss
+ * and weight_sum are needed. */
 int bsi_b200_distill_fused(const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan,
                            const int64_t* ids, const void* teacher, int teacher_dtype, int K, float temperature, int tail,
                            const float* weights, int mean, float* row_loss, float* loss, float* weight_sum,

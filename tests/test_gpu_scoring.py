@@ -30,6 +30,9 @@ def rows_of(kind, rows, V, dtype, seed):
         keep = torch.rand(rows, V, generator=g) < 0.5
         keep[:, V // 2] = True
         z = torch.where(keep, z, torch.tensor(torch.finfo(dtype).min))
+    elif kind == "only lowest":        # nothing but the lowest value and -inf
+        z = torch.where(torch.rand(rows, V, generator=g) < 0.5, torch.tensor(torch.finfo(dtype).min), torch.tensor(-float("inf")))
+        z[:, V // 2] = torch.finfo(dtype).min
     elif kind == "far":                # one entry far above the rest, and levels far from zero
         z = z * 4 + 200.0
         z[:, V // 3] += 60.0
@@ -81,7 +84,7 @@ def test_sizes(dtype, rows, V, k):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
-@pytest.mark.parametrize("kind", ["ties", "constant", "masked", "lowest", "far"])
+@pytest.mark.parametrize("kind", ["ties", "constant", "masked", "lowest", "only lowest", "far"])
 @pytest.mark.parametrize("rows,V,k", [(2, 300, 20), (3, 9001, 128), (1, 50272, 64)])
 def test_contents(kind, dtype, rows, V, k):
     z = rows_of(kind, rows, V, DT[dtype], V)
