@@ -4,8 +4,8 @@
 // tcgen05.mma.kind::mxf4 / mxf4nvf4 multiplies the codes and both block scales itself (K = 64 per instruction) and accumulates in
 // float32 in TMEM; what is left for the epilogue are the per-row factors of the nvfp4 format, the bias, ReLU and one rounding.
 //
-// The weights' rows are the instruction's M (128 TMEM lanes), the tokens its N: one form serves one token (N = 16) and a prompt
-// (N = 256), and a warp of the epilogue stores 32 neighbouring outputs of a token.
+// The weights' rows are the instruction's M (TMEM lanes), the tokens its N, so that one token takes the same way as a prompt, and a
+// warp of the epilogue stores 32 neighbouring outputs of a token. Up to 128 tokens, a CTA by itself with all of them (fp4_linear_kernel):
 //
 //   warp 0     TMA producer: per k-block of 256 elements one box of weights (128 x 128 B), one of tokens (BN x 128 B), both 128-byte
 //              swizzled, and their scales as they lie in memory (512 bytes for 128 rows x 4 scales, whole tiles)
@@ -50,19 +50,18 @@ constexpr int kSiteBase = 128;         // of the status word: sites 129 and up a
 template <int BN, bool MX>
 struct Cfg {
     static constexpr int kGroups = MX ? 2 : 4;                   // scale tiles of a k-block per 128 rows
-    static constexpr int kNTiles = BN > 128 ? 2 : 1;             // scale row tiles that BN tokens lie in
     static constexpr int kWBytes = kTileM * kRowBytes;
     static constexpr int kXBytes = BN * kRowBytes;
     static constexpr int kWScale = kGroups * kScaleTile;
-    static constexpr int kXScale = kNTiles * kGroups * kScaleTile;
+    static constexpr int kXScale = kGroups * kScaleTile;
     static constexpr int kStageBytes = kWBytes + kXBytes + kWScale + kXScale;      // a multiple of 1 KB
     // two CTAs per SM for the narrow tiles, whose MMAs are short beside their loads
     static constexpr int kPerSm = BN <= 64 ? 2 : 1;
     static constexpr int kBudget = (kPerSm == 2 ? 113 : 226) * 1024 - 2048;
     static constexpr int kStages = kBudget / kStageBytes > 8 ? 8 : kBudget / kStageBytes;
-    static constexpr int kSmem = kStages * kStageBytes + (2 * kStages + 2) * 8 + 32 + 1024;
+    static constexpr int kSmem = kStages * kStageBytes + (2 * kStages + 2) * 8 + 32 + BN * 4 + 1024;
     // TMEM: the accumulator, then two sets of scales (4 columns for each tile of 512 bytes)
-    static constexpr int kScaleCols = 4 * kGroups * (1 + kNTiles);
+    static constexpr int kScaleCols = 4 * kGroups * 2;
     static constexpr int kScale0 = BN < 32 ? 32 : BN;
     static constexpr int kNeed = kScale0 + 2 * kScaleCols;
     static constexpr int kTmemCols = kNeed <= 128 ? 128 : (kNeed <= 256 ? 256 : 512);
@@ -147,6 +146,13 @@ template <> __device__ __forceinline__ float narrow<float>(float v) { return v; 
 template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// One rounding, to the output's type.
+template <typename T>
+__device__ __forceinline__ T finished(float sum, float factor, float bias, int relu) {
+    const float v = __fmaf_rn(sum, factor, bias);
+    return narrow<T>(relu && v < 0.0f ? 0.0f : v);
+}
+
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -175,6 +181,7 @@ __global__ void __launch_bounds__(kThreads) fp4_linear_kernel(const __grid_const
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * C::kStageBytes);      // full[], empty[], done, drain
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* token_scale = reinterpret_cast<float*>(tmem_slot + 4);      // BN
     const uint32_t base = smem_u32(smem), bar0 = smem_u32(bars);
     auto full = [&](int s) { return bar0 + 8u * s; };
     auto empty = [&](int s) { return bar0 + 8u * (kStages + s); };
@@ -183,7 +190,6 @@ __global__ void __launch_bounds__(kThreads) fp4_linear_kernel(const __grid_const
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int parts = static_cast<int>(cluster_size()), part = static_cast<int>(cluster_rank());
     const int n0 = static_cast<int>(blockIdx.x) / parts * kTileM;      // first output (row of the weights)
-    const int m0 = static_cast<int>(blockIdx.y) * BN;                  // first token
     const int kb0 = static_cast<int>(static_cast<int64_t>(a.blocks) * part / parts);
     const int kb1 = static_cast<int>(static_cast<int64_t>(a.blocks) * (part + 1) / parts);
     const int count = kb1 - kb0;
@@ -212,26 +218,21 @@ __global__ void __launch_bounds__(kThreads) fp4_linear_kernel(const __grid_const
 
     if (warp == 0) {
         if (lane == 0) {
-            // the tokens' scale tiles that are there (the last column tile may end in the first)
-            const int x_tiles = C::kNTiles == 2 && m0 + 128 < a.M ? 2 : 1;
-            const uint32_t bytes = static_cast<uint32_t>(C::kWBytes + C::kXBytes + C::kWScale + x_tiles * C::kGroups * kScaleTile);
             const int64_t groups = static_cast<int64_t>(a.blocks) * C::kGroups;
             const uint8_t* ws = a.w_scales + (n0 / 128) * groups * kScaleTile;
-            const uint8_t* xs = a.x_scales + (m0 / 128) * groups * kScaleTile;
+            const uint8_t* xs = a.x_scales;        // of the one row tile
             auto load_w = [&](int i) {
                 const int s = i % kStages;
                 const uint32_t dst = base + s * C::kStageBytes;
-                mbar_expect_tx(full(s), bytes);
+                mbar_expect_tx(full(s), C::kStageBytes);
                 tma_load_2d(dst, &map_w, (kb0 + i) * kRowBytes, n0, full(s));
                 bulk_load(dst + C::kWBytes + C::kXBytes, ws + static_cast<int64_t>(kb0 + i) * C::kWScale, C::kWScale, full(s));
             };
             auto load_x = [&](int i) {
                 const int s = i % kStages;
                 const uint32_t dst = base + s * C::kStageBytes;
-                tma_load_2d(dst + C::kWBytes, &map_x, (kb0 + i) * kRowBytes, m0, full(s));
-                for (int t = 0; t < x_tiles; ++t)
-                    bulk_load(dst + C::kWBytes + C::kXBytes + C::kWScale + t * C::kGroups * kScaleTile,
-                              xs + (t * groups + static_cast<int64_t>(kb0 + i) * C::kGroups) * kScaleTile, C::kGroups * kScaleTile, full(s));
+                tma_load_2d(dst + C::kWBytes, &map_x, (kb0 + i) * kRowBytes, 0, full(s));
+                bulk_load(dst + C::kWBytes + C::kXBytes + C::kWScale, xs + static_cast<int64_t>(kb0 + i) * C::kXScale, C::kXScale, full(s));
             };
             // the weights come from before the packer: a ring of them ahead of the wait for it
             const int ahead = a.dependent ? min(kStages, count) : 0;
@@ -268,16 +269,13 @@ __global__ void __launch_bounds__(kThreads) fp4_linear_kernel(const __grid_const
 #pragma unroll
                 for (int g = 0; g < C::kGroups; ++g) {
                     copy_scales(ca + 4 * g, scale_desc(sa + g * kScaleTile));
-#pragma unroll
-                    for (int t = 0; t < C::kNTiles; ++t)      // the columns of one group behind one another, 128 tokens each
-                        copy_scales(cb + 4 * (g * C::kNTiles + t), scale_desc(sb + (t * C::kGroups + g) * kScaleTile));
+                    copy_scales(cb + 4 * g, scale_desc(sb + g * kScaleTile));
                 }
                 const uint64_t da = umma_desc(wa), db = umma_desc(xa);
-                const uint32_t col = BN < 128 ? (m0 % 128) / 32 : 0;      // tokens 32 to a column
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int g = MX ? k >> 1 : k;
-                    umma_fp4<MX>(tmem, da + 2u * k, db + 2u * k, instruction<MX>(BN, MX ? (k & 1) * 2 : 0), ca + 4 * g, cb + 4 * g * C::kNTiles + col,
+                    umma_fp4<MX>(tmem, da + 2u * k, db + 2u * k, instruction<MX>(BN, MX ? (k & 1) * 2 : 0), ca + 4 * g, cb + 4 * g,
                                  (i | k) != 0 ? 1u : 0u);
                 }
                 umma_commit(empty(s));
@@ -307,28 +305,25 @@ __global__ void __launch_bounds__(kThreads) fp4_linear_kernel(const __grid_const
             if (a.bias != nullptr) bias = a.bias[n];
         }
         if (a.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
+        for (int c = threadIdx.x - 64; c < BN; c += kThreads - 64) token_scale[c] = a.x_row != nullptr && c < a.M ? *behind_wait(a.x_row + c) : 1.0f;
+        asm volatile("bar.sync 1, 128;" ::: "memory");       // the four epilogue warps
         ok = __all_sync(0xFFFFFFFFu, wait_for(done, 0, abort_flag, 3));
         tc_fence_after();
     }
-    auto store = [&](float v, int m) {
-        if (m < a.M && n < a.N) {
-            const float gx = a.x_row != nullptr ? a.x_row[m] : 1.0f;
-            v = __fmaf_rn(v, gw * gx, bias);
-            if (a.relu && v < 0.0f) v = 0.0f;
-            y[static_cast<int64_t>(m) * a.ldy + n] = narrow<OutT>(v);
-        }
+    auto store = [&](float v, int c) {
+        if (c < a.M && n < a.N) y[c * a.ldy + n] = finished<OutT>(v, gw * token_scale[c], bias, a.relu);
     };
     if (epi && ok) {
         const uint32_t at = tmem + (static_cast<uint32_t>(quad * 32) << 16);
         constexpr int kPiece = BN < 32 ? 16 : 32;
-        for (int c = 0; c < BN && m0 + c < a.M; c += kPiece) {
+        for (int c = 0; c < BN && c < a.M; c += kPiece) {
             int32_t v[32];
             if constexpr (BN < 32) tmem_ld16(at + c, v);
             else tmem_ld32(at + c, v);
             tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < kPiece; ++e) {
-                if (parts == 1) store(__int_as_float(v[e]), m0 + c + e);
+                if (parts == 1) store(__int_as_float(v[e]), c + e);
                 else sums[(c + e) * kTileM + feature] = __int_as_float(v[e]);
             }
         }
@@ -338,10 +333,10 @@ __global__ void __launch_bounds__(kThreads) fp4_linear_kernel(const __grid_const
         if (epi && ok) {
             // tokens beyond M have no sums; an aborted part leaves its ring's contents, and the status word tells
             const int lo = BN * part / parts, hi = BN * (part + 1) / parts;
-            for (int c = lo; c < hi && m0 + c < a.M; ++c) {
+            for (int c = lo; c < hi && c < a.M; ++c) {
                 float v = 0.0f;
                 for (int p = 0; p < parts; ++p) v += remote_float(smem_u32(sums + c * kTileM + feature), static_cast<uint32_t>(p));
-                store(v, m0 + c);
+                store(v, c);
             }
         }
         cluster_sync();      // the others read this CTA's sums
@@ -351,6 +346,285 @@ __global__ void __launch_bounds__(kThreads) fp4_linear_kernel(const __grid_const
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(static_cast<uint32_t>(C::kTmemCols)) : "memory");
+    }
+}
+
+// ---- more than 128 tokens: paired CTAs ------------------------------------------------------------------------------------------
+//
+// A pair of CTAs (tcgen05 cta_group::2) works on 256 outputs x BN tokens: each CTA loads its own 128 rows of the weights, half of the
+// tokens and the scales that its tensor core reads, its own weights' and all the tokens'. 38 KB a k-block and CTA for 512 cycles of
+// MMAs at BN = 256; a CTA by itself with a tile of 128 x 256 would load 54 KB, and the way from L2 to an SM carries about 64 bytes a cycle.
+// Persistent: pairs walk over the tiles, loads run ahead into the next one, and the epilogue takes a finished accumulator into registers
+// in one go (8 warps, BN / 2 columns each), hands TMEM back and stores while the next tile's MMAs run.
+//   warp 0     TMA producer (both CTAs; every load signals the leader's barrier)
+//   warp 1     TMEM; MMA issuer (leader)
+//   warps 4-11 epilogue (both CTAs)
+constexpr int kPairThreads = 384;
+
+template <int BN, bool MX>
+struct PairCfg {
+    static constexpr int kGroups = MX ? 2 : 4;
+    static constexpr int kNTiles = BN / 128;
+    static constexpr int kWBytes = kTileM * kRowBytes;
+    static constexpr int kXBytes = BN / 2 * kRowBytes;
+    static constexpr int kWScale = kGroups * kScaleTile;
+    static constexpr int kXScale = kNTiles * kGroups * kScaleTile;
+    static constexpr int kStageBytes = kWBytes + kXBytes + kWScale + kXScale;
+    static constexpr int kFixed = 8 * (BN / 2) * 4 + 256 + 1024;      // token factors of the 8 epilogue warps, barriers and slots, alignment
+    static constexpr int kFit = (232448 - kFixed) / kStageBytes;
+    static constexpr int kStages = kFit > 8 ? 8 : kFit;
+    static constexpr int kSmem = kStages * kStageBytes + kFixed;
+    static constexpr int kScaleCols = 4 * kGroups * (1 + kNTiles);
+    static constexpr int kTmemCols = 512;
+    static_assert(kStageBytes % 1024 == 0 && kStages >= 4 && BN + 2 * kScaleCols <= kTmemCols && (2 * kStages + 3) * 8 + 16 <= 256, "does not fit");
+};
+
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t leader_bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(leader_bar)
+                 : "memory");
+}
+// Each CTA's scales from its own shared memory into its own TMEM.
+__device__ __forceinline__ void copy_scales_pair(uint32_t tmem, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+template <bool MX>
+__device__ __forceinline__ void umma_fp4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    if constexpr (MX) {
+        asm volatile(
+            "{\n.reg .pred p;\n"
+            "setp.ne.b32 p, %6, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+    } else {
+        asm volatile(
+            "{\n.reg .pred p;\n"
+            "setp.ne.b32 p, %6, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+    }
+}
+// Arrives on the barrier at this offset in both CTAs once all earlier MMAs are done.
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+// M = 256 over the pair.
+template <bool MX>
+__host__ __device__ constexpr uint32_t instruction_pair(int n, int pair) {
+    return (instruction<MX>(n, pair) & ~(3u << 27)) | (2u << 27);
+}
+
+struct PairArgs {
+    const float* w_row;
+    const float* x_row;
+    const float* bias;
+    void* y;
+    int64_t ldy;
+    int M, N, blocks, relu, dependent;
+    int tiles_n, tiles;      // tiles along the outputs, in all
+};
+
+// A wait that, when it gives up, ends both CTAs' work.
+struct PairWait {
+    volatile int* flag;
+    uint32_t peer_flag;
+    __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity, int site) const {
+        if (mbar_try(bar, parity)) return true;
+        const long long t0 = clock64();
+        for (;;) {
+            if (mbar_try_parked(bar, parity, 20000u)) return true;
+            if (*flag) return false;
+            if (clock64() - t0 > kWaitCycles) {
+                *flag = 1;
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_flag), "r"(1) : "memory");
+                atomicCAS(&g_fp4_status, 0, kSiteBase + site);
+                return false;
+            }
+        }
+    }
+};
+
+template <int BN, bool MX, typename OutT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    fp4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_ws,
+                    const __grid_constant__ CUtensorMap map_xs, const PairArgs a) {
+    using C = PairCfg<BN, MX>;
+    constexpr int kStages = C::kStages;
+    constexpr int kCols = BN / 2;        // columns of an epilogue warp
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * C::kStageBytes);      // full[], empty[], tfull, tempty, drained
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 3);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* token_scale = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);      // [8][kCols]
+    const uint32_t base = smem_u32(smem), bar0 = smem_u32(bars);
+    auto full = [&](int s) { return bar0 + 8u * s; };
+    auto empty = [&](int s) { return bar0 + 8u * (kStages + s); };
+    const uint32_t tfull = bar0 + 8u * (2 * kStages), tempty = tfull + 8u, drained = tfull + 16u;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int first = static_cast<int>(blockIdx.x) / 2, step = static_cast<int>(gridDim.x) / 2;
+    const PairWait wait{abort_flag, in_cta(smem_u32(const_cast<int*>(abort_flag)), rank ^ 1u)};
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        mbar_init(tfull, 1);
+        mbar_init(tempty, 16);       // the epilogue warps of both CTAs, at the leader's
+        mbar_init(drained, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(tmem_slot)), "r"(static_cast<uint32_t>(C::kTmemCols)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            if (a.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
+            int s = 0, issued = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = first; t < a.tiles && ok; t += step) {
+                const int n0 = t % a.tiles_n * 256, m0 = t / a.tiles_n * BN;
+                for (int kb = 0; kb < a.blocks; ++kb) {
+                    if (!wait(empty(s), phase ^ 1u, 1)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t dst = base + s * C::kStageBytes, bar = in_cta(full(s), 0);
+                    if (rank == 0) mbar_expect_tx(full(s), 2 * C::kStageBytes);
+                    tma_load_pair(dst, &map_w, kb * kRowBytes, n0 + static_cast<int>(rank) * 128, bar);
+                    tma_load_pair(dst + C::kWBytes, &map_x, kb * kRowBytes, m0 + static_cast<int>(rank) * (BN / 2), bar);
+                    // tiles of 512 bytes are the rows of the scales' maps; a row tile beyond the last reads as zeros
+                    const uint32_t sc = dst + C::kWBytes + C::kXBytes;
+                    tma_load_pair(sc, &map_ws, 0, ((n0 >> 7) + static_cast<int>(rank)) * a.blocks * C::kGroups + kb * C::kGroups, bar);
+#pragma unroll
+                    for (int q = 0; q < C::kNTiles; ++q)
+                        tma_load_pair(sc + C::kWScale + q * C::kGroups * kScaleTile, &map_xs, 0, ((m0 >> 7) + q) * a.blocks * C::kGroups + kb * C::kGroups, bar);
+                    ++issued;
+                    if (++s == kStages) {
+                        s = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            if (!ok && rank == 0) {
+                // let what was issued land (bounded); the barriers that count are the leader's
+                for (int i = max(0, issued - kStages); i < issued; ++i) drain(full(i % kStages), static_cast<uint32_t>(i / kStages) & 1u);
+            }
+        }
+    } else if (warp == 1 && rank == 0) {
+        if (lane == 0) {
+            int s = 0, count = 0;
+            uint32_t phase = 0, tphase = 0;
+            bool ok = true;
+            for (int t = first; t < a.tiles && ok; t += step) {
+                if (!wait(tempty, tphase ^ 1u, 2)) {
+                    ok = false;
+                    break;
+                }
+                tphase ^= 1u;
+                tc_fence_after();
+                for (int kb = 0; kb < a.blocks; ++kb) {
+                    if (!wait(full(s), phase, 3)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t wa = base + s * C::kStageBytes, xa = wa + C::kWBytes, sa = xa + C::kXBytes, sb = sa + C::kWScale;
+                    const uint32_t ca = tmem + BN + (count & 1) * C::kScaleCols, cb = ca + 4 * C::kGroups;
+#pragma unroll
+                    for (int g = 0; g < C::kGroups; ++g) {
+                        copy_scales_pair(ca + 4 * g, scale_desc(sa + g * kScaleTile));
+#pragma unroll
+                        for (int q = 0; q < C::kNTiles; ++q)
+                            copy_scales_pair(cb + 4 * (g * C::kNTiles + q), scale_desc(sb + (q * C::kGroups + g) * kScaleTile));
+                    }
+                    const uint64_t da = umma_desc(wa), db = umma_desc(xa);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int g = MX ? k >> 1 : k;
+                        umma_fp4_pair<MX>(tmem, da + 2u * k, db + 2u * k, instruction_pair<MX>(BN, MX ? (k & 1) * 2 : 0), ca + 4 * g,
+                                          cb + 4 * g * C::kNTiles, (kb | k) != 0 ? 1u : 0u);
+                    }
+                    commit_pair(empty(s));
+                    ++count;
+                    if (++s == kStages) {
+                        s = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (ok) commit_pair(tfull);
+            }
+            if (!ok) {
+                commit_pair(drained);
+                drain(drained, 0);
+            }
+        }
+    } else if (warp >= 4) {
+        const int quad = warp & 3, half = (warp - 4) >> 2;
+        if (a.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
+        const uint32_t leader_tempty = in_cta(tempty, 0);
+        uint32_t phase = 0;
+        float* scale = token_scale + (warp - 4) * kCols;
+        for (int t = first; t < a.tiles; t += step) {
+            const int n = t % a.tiles_n * 256 + static_cast<int>(rank) * 128 + quad * 32 + lane, m0 = t / a.tiles_n * BN;
+            // what the tile needs beside its sums, while the MMAs run
+            const int m = m0 + half * kCols;
+            __syncwarp();
+            for (int c = lane; c < kCols; c += 32) scale[c] = a.x_row != nullptr && m + c < a.M ? *behind_wait(a.x_row + m + c) : 1.0f;
+            const float gw = a.w_row != nullptr && n < a.N ? a.w_row[n] : 1.0f, bias = a.bias != nullptr && n < a.N ? a.bias[n] : 0.0f;
+            __syncwarp();
+            if (!__all_sync(0xFFFFFFFFu, wait(tfull, phase, 4))) break;
+            phase ^= 1u;
+            tc_fence_after();
+            int32_t v[kCols / 32][32];
+            const uint32_t at = tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * kCols;
+#pragma unroll
+            for (int q = 0; q < kCols / 32; ++q) tmem_ld32(at + q * 32, v[q]);
+#pragma unroll
+            for (int q = 0; q < kCols / 32; ++q) tmem_ld_wait_for(v[q]);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(leader_tempty) : "memory");
+            const int tokens = min(kCols, a.M - m);
+            if (n < a.N) {
+                OutT* y = static_cast<OutT*>(a.y) + static_cast<int64_t>(m) * a.ldy + n;
+                if (tokens == kCols) {
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c, y += a.ldy) *y = finished<OutT>(__int_as_float(v[c / 32][c % 32]), gw * scale[c], bias, a.relu);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c, y += a.ldy)
+                        if (c < tokens) *y = finished<OutT>(__int_as_float(v[c / 32][c % 32]), gw * scale[c], bias, a.relu);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();      // the other CTA's MMAs read this one's shared memory, its warps signal this one's barriers
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(static_cast<uint32_t>(C::kTmemCols)) : "memory");
     }
 }
 
@@ -390,10 +664,10 @@ int launch(const Operands& o, const Args& a, cudaStream_t stream) {
     int rc = make_codes_map(&mw, o.w, a.N, bytes, o.ldw, kTileM);
     if (rc == BSI_OK) rc = make_codes_map(&mx, o.x, a.M, bytes, o.ldx, BN);
     if (rc != BSI_OK) return rc;
-    const int tiles_n = (a.N + kTileM - 1) / kTileM, tiles_m = (a.M + BN - 1) / BN;
+    const int tiles_n = (a.N + kTileM - 1) / kTileM;
     const int64_t slots = static_cast<int64_t>(C::kPerSm) * sm_count();
     int parts = 1;
-    while (parts < 8 && static_cast<int64_t>(tiles_n) * tiles_m * parts * 2 <= slots && a.blocks >= parts * 4) parts *= 2;
+    while (parts < 8 && static_cast<int64_t>(tiles_n) * parts * 2 <= slots && a.blocks >= parts * 4) parts *= 2;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -401,7 +675,7 @@ int launch(const Operands& o, const Args& a, cudaStream_t stream) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(tiles_n * parts), static_cast<unsigned>(tiles_m), 1);
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles_n * parts), 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
     cfg.dynamicSmemBytes = C::kSmem;
     cfg.stream = stream;
@@ -415,13 +689,71 @@ int launch(const Operands& o, const Args& a, cudaStream_t stream) {
     return BSI_OK;
 }
 
+// The scales as rows of 512 bytes, `groups` of them a box.
+int make_scales_map(CUtensorMap* map, const uint8_t* scales, int64_t tiles, int groups) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (fn == nullptr) return fail(BSI_ERR_CUDA, "fp4_linear: cuTensorMapEncodeTiled entry point not found");
+    const cuuint64_t dims[2] = {kScaleTile / 4, static_cast<cuuint64_t>(tiles)};
+    const cuuint64_t strides[1] = {kScaleTile};
+    const cuuint32_t box[2] = {kScaleTile / 4, static_cast<cuuint32_t>(groups)};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<uint8_t*>(scales), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("fp4_linear: cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(r));
+        return BSI_ERR_CUDA;
+    }
+    return BSI_OK;
+}
+
+template <int BN, bool MX, typename OutT>
+int launch_pair(const Operands& o, const Args& a, cudaStream_t stream) {
+    using C = PairCfg<BN, MX>;
+    static bool attr_set[64] = {false};
+    int dev = 0;
+    BSI_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+        BSI_CUDA_TRY(cudaFuncSetAttribute(fp4_pair_kernel<BN, MX, OutT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+        if (dev >= 0 && dev < 64) attr_set[dev] = true;
+    }
+    CUtensorMap mw, mx, mws, mxs;
+    const int64_t bytes = (o.K + 31) / 32 * 16, per_row_tile = static_cast<int64_t>(a.blocks) * C::kGroups;
+    int rc = make_codes_map(&mw, o.w, a.N, bytes, o.ldw, kTileM);
+    if (rc == BSI_OK) rc = make_codes_map(&mx, o.x, a.M, bytes, o.ldx, BN / 2);
+    if (rc == BSI_OK) rc = make_scales_map(&mws, a.w_scales, (a.N + 127ll) / 128 * per_row_tile, C::kGroups);
+    if (rc == BSI_OK) rc = make_scales_map(&mxs, a.x_scales, (a.M + 127ll) / 128 * per_row_tile, C::kGroups);
+    if (rc != BSI_OK) return rc;
+    PairArgs p{a.w_row, a.x_row, a.bias, a.y, a.ldy, a.M, a.N, a.blocks, a.relu, a.dependent, (a.N + 255) / 256, 0};
+    p.tiles = p.tiles_n * ((a.M + BN - 1) / BN);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min(p.tiles, sm_count() / 2)), 1, 1);
+    cfg.blockDim = dim3(kPairThreads, 1, 1);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.dependent ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, fp4_pair_kernel<BN, MX, OutT>, mw, mx, mws, mxs, p);
+    if (e != cudaSuccess) {
+        set_error("fp4_linear launch: %s", cudaGetErrorString(e));
+        return BSI_ERR_CUDA;
+    }
+    return BSI_OK;
+}
+
 template <bool MX, typename OutT>
 int launch_width(const Operands& o, const Args& a, cudaStream_t stream) {
     if (a.M <= 16) return launch<16, MX, OutT>(o, a, stream);
     if (a.M <= 32) return launch<32, MX, OutT>(o, a, stream);
     if (a.M <= 64) return launch<64, MX, OutT>(o, a, stream);
     if (a.M <= 128) return launch<128, MX, OutT>(o, a, stream);
-    return launch<256, MX, OutT>(o, a, stream);
+    // rounds of the GPU's pairs over tiles of 256 or 128 tokens; a narrow tile's MMAs are half as long, its loads three quarters
+    const int64_t pairs = sm_count() / 2, outputs = (a.N + 255) / 256;
+    const int64_t wide = (outputs * ((a.M + 255) / 256) + pairs - 1) / pairs, narrow_ = (outputs * ((a.M + 127) / 128) + pairs - 1) / pairs;
+    if (wide * 4 <= narrow_ * 3) return launch_pair<256, MX, OutT>(o, a, stream);
+    return launch_pair<128, MX, OutT>(o, a, stream);
 }
 
 template <bool MX>
