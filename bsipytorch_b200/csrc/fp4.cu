@@ -31,39 +31,58 @@ __device__ __forceinline__ float widen(float v) { return v; }
 __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
 __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// 16 elements from column c of a row, zero behind column K.
+// 16 elements as they lie in memory, zero behind column K.
 template <typename T>
-__device__ __forceinline__ void load_unit(const T* row, int64_t c, int64_t K, bool vector, float (&x)[kUnit]) {
-    constexpr int kVec = 16 / sizeof(T);
-    if (vector && c + kUnit <= K) {
+struct Unit {
+    static constexpr int kVecs = kUnit * sizeof(T) / 16;
+    uint4 u[kVecs];
+
+    __device__ __forceinline__ void load(const T* row, int64_t c, int64_t K, bool vector) {
+        if (vector && c + kUnit <= K) {
 #pragma unroll
-        for (int i = 0; i < kUnit / kVec; ++i) {
-            const uint4 u = *reinterpret_cast<const uint4*>(row + c + i * kVec);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            for (int i = 0; i < kVecs; ++i) u[i] = *reinterpret_cast<const uint4*>(row + c + i * (16 / sizeof(T)));
+        } else {
+            T* e = reinterpret_cast<T*>(u);
+#pragma unroll
+            for (int i = 0; i < kUnit; ++i) e[i] = c + i < K ? row[c + i] : static_cast<T>(0.0f);
+        }
+    }
+    // Largest magnitude as a float32's bits: the order of non-negative floats, infinities and NaN above all.
+    __device__ __forceinline__ uint32_t magnitude() const {
+        if constexpr (sizeof(T) == 4) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) m = max(max(m, max(u[i].x & 0x7FFFFFFFu, u[i].y & 0x7FFFFFFFu)), max(u[i].z & 0x7FFFFFFFu, u[i].w & 0x7FFFFFFFu));
+            return m;
+        } else {
+            // both halves of a word at once: a sign bit less, 16-bit patterns are in the order of their magnitudes
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) {
+                m = __vmaxu2(m, __vmaxu2(u[i].x & 0x7FFF7FFFu, u[i].y & 0x7FFF7FFFu));
+                m = __vmaxu2(m, __vmaxu2(u[i].z & 0x7FFF7FFFu, u[i].w & 0x7FFF7FFFu));
+            }
+            const unsigned short top = static_cast<unsigned short>(max(m & 0xFFFFu, m >> 16));
+            return __float_as_uint(widen(*reinterpret_cast<const T*>(&top)));
+        }
+    }
+    __device__ __forceinline__ void values(float (&x)[kUnit]) const {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            const uint32_t word[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if constexpr (sizeof(T) == 4) {
-                    x[i * 4 + j] = __uint_as_float(w[j]);
+                    x[i * 4 + j] = __uint_as_float(word[j]);
                 } else {
-                    const T* p = reinterpret_cast<const T*>(&w[j]);
+                    const T* p = reinterpret_cast<const T*>(&word[j]);
                     x[i * 8 + j * 2] = widen(p[0]);
                     x[i * 8 + j * 2 + 1] = widen(p[1]);
                 }
             }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < kUnit; ++i) x[i] = c + i < K ? widen(row[c + i]) : 0.0f;
     }
-}
-
-// Largest magnitude as a bit pattern: the order of non-negative floats, infinities and NaN above all.
-__device__ __forceinline__ uint32_t magnitude(const float (&x)[kUnit]) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < kUnit; ++i) m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-    return m;
-}
+};
 
 // Two e2m1 codes, lo in the lower nibble; four such bytes.
 __device__ __forceinline__ uint32_t codes8(const float* v) {
@@ -79,12 +98,18 @@ __device__ __forceinline__ uint32_t codes8(const float* v) {
     return r;
 }
 
-// x / scale correctly rounded where the quotient is no smaller than 2^-100 (a smaller one is no border's neighbour): the residual of
-// the first guess is exact in a fused multiply-add, and one step with a correctly rounded reciprocal ends at the rounded quotient
-// (Markstein's theorem; the scale's significand has four bits).
-__device__ __forceinline__ float quotient(float x, float scale, float inv) {
-    const float q = __fmul_rn(x, inv);
-    return __fmaf_rn(__fmaf_rn(-q, scale, x), inv, q);
+// x / scale correctly rounded where the quotient is no smaller than 2^-100 (a smaller one is no border's neighbour), two at a time: the
+// residual of the first guess is exact in a fused multiply-add, and one step with a correctly rounded reciprocal ends at the rounded
+// quotient (Markstein's theorem; the scale's significand has four bits).
+__device__ __forceinline__ void quotients(float& x, float& y, float scale, float inv) {
+    unsigned long long v, s, i, q, r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    asm("mov.b64 %0, {%1, %1};" : "=l"(s) : "f"(-scale));
+    asm("mov.b64 %0, {%1, %1};" : "=l"(i) : "f"(inv));
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(q) : "l"(v), "l"(i));
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(q), "l"(s), "l"(v));
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(q) : "l"(r), "l"(i), "l"(q));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(q));
 }
 
 __device__ __forceinline__ uint32_t e4m3_byte(float v) {
@@ -98,36 +123,43 @@ __device__ __forceinline__ float power_of_two(int e) {
     return e >= -126 ? __uint_as_float(static_cast<uint32_t>(e + 127) << 23) : __uint_as_float(1u << (e + 149));
 }
 
+// One row a CTA. What bounds it is the matrix's bytes; a row's maximum has to be known before its first code, so a thread keeps up to
+// two units as they came (beyond 16384 columns the rest is read again), and what fills the wait are other rows: 64 bytes of a unit's
+// row, not 16 float32 values, keep the registers low enough for it (8192 x 4096 bfloat16 nvfp4: 71 us with 92 registers).
 template <typename T, bool MX>
-__global__ void __launch_bounds__(kMaxThreads) fp4_quantize_kernel(const T* __restrict__ x, int64_t K, int64_t ldx, int vector, uint8_t* __restrict__ codes,
-                                                                   int64_t ld, uint8_t* __restrict__ scales, float* __restrict__ row_scale) {
+__global__ void __launch_bounds__(kMaxThreads, sizeof(T) == 4 ? 2 : 3)
+    fp4_quantize_kernel(const T* __restrict__ x, int64_t K, int64_t ldx, int vector, uint8_t* __restrict__ codes, int64_t ld, uint8_t* __restrict__ scales,
+                        float* __restrict__ row_scale) {
     __shared__ uint32_t part[kMaxThreads / 32];
-    const int64_t r = blockIdx.x;
+    const uint32_t r = blockIdx.x;
     const T* row = x + r * ldx;
-    const int64_t units = (K + 255) / 256 * 16;              // also those whose scales are there without elements
-    const int64_t groups = units / (MX ? 8 : 4);
-    float held[MX ? 1 : kHeld][kUnit];
+    const int units = static_cast<int>((K + 255) / 256 * 16);       // also those whose scales are there without elements
+    const int groups = units / (MX ? 8 : 4);
+    const int threads = static_cast<int>(blockDim.x);
     float g = 1.0f;
     bool finite = true;
+    Unit<T> held[kHeld];
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h) {
+        const int u = static_cast<int>(threadIdx.x) + h * threads;
+        if (u < units) held[h].load(row, static_cast<int64_t>(u) * kUnit, K, vector != 0);
+    }
     if constexpr (!MX) {
         uint32_t top = 0;
 #pragma unroll
-        for (int h = 0; h < kHeld; ++h) {
-            const int64_t u = threadIdx.x + static_cast<int64_t>(h) * blockDim.x;
-            if (u < units) {
-                load_unit(row, u * kUnit, K, vector != 0, held[h]);
-                top = max(top, magnitude(held[h]));
-            }
-        }
-        for (int64_t u = threadIdx.x + static_cast<int64_t>(kHeld) * blockDim.x; u < units; u += blockDim.x) {
-            float v[kUnit];
-            load_unit(row, u * kUnit, K, vector != 0, v);
-            top = max(top, magnitude(v));
+        for (int h = 0; h < kHeld; ++h)
+            if (static_cast<int>(threadIdx.x) + h * threads < units) top = max(top, held[h].magnitude());
+        for (int u = static_cast<int>(threadIdx.x) + kHeld * threads; u < units; u += threads) {
+            Unit<T> v;
+            v.load(row, static_cast<int64_t>(u) * kUnit, K, vector != 0);
+            top = max(top, v.magnitude());
         }
         top = __reduce_max_sync(0xFFFFFFFFu, top);
-        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
-        __syncthreads();
-        for (unsigned w = 0; w < blockDim.x / 32; ++w) top = max(top, part[w]);
+        if (threads > 32) {
+            if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+            __syncthreads();
+            for (int w = 0; w < threads / 32; ++w) top = max(top, part[w]);
+        }
         finite = top < 0x7F800000u;
         if (finite && top != 0) {
             // the smallest e with top <= 2688 * 2^e = 1.3125 * 2^(11 + e)
@@ -137,56 +169,53 @@ __global__ void __launch_bounds__(kMaxThreads) fp4_quantize_kernel(const T* __re
         if (threadIdx.x == 0) row_scale[r] = finite ? g : __uint_as_float(0x7FC00000u);
     }
     uint8_t* crow = codes + r * ld;
-    uint8_t* stile = scales + (r / 128) * groups * 512 + (r % 32) * 16 + (r % 128) / 32 * 4;
+    uint8_t* stile = scales + static_cast<int64_t>(r / 128) * groups * 512 + (r % 32) * 16 + (r % 128) / 32 * 4;
     const float six_g = 6.0f * g;
-    int h = 0;
-    const int64_t passes = (units + blockDim.x - 1) / blockDim.x;
-    for (int64_t p = 0; p < passes; ++p, ++h) {
-        const int64_t u = threadIdx.x + p * blockDim.x;
-        float v[kUnit];
-        uint32_t m = 0;
-        const bool live = u < units;
-        if (live) {
-            bool have = false;
-            if constexpr (!MX) {
-#pragma unroll
-                for (int i = 0; i < kHeld; ++i) {
-                    if (h == i) {
-#pragma unroll
-                        for (int e = 0; e < kUnit; ++e) v[e] = held[i][e];
-                        have = true;
-                    }
-                }
-            }
-            if (!have) load_unit(row, u * kUnit, K, vector != 0, v);
-            m = magnitude(v);
-        }
+    auto pack = [&](const Unit<T>& unit, int u, bool live) {
+        uint32_t m = live ? unit.magnitude() : 0u;
         float scale, inv;
         uint32_t byte;
         if constexpr (MX) {
             m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));            // the block's other half
             // e8m0: the exponent of amax less 2 under the bias of 127; not finite: NaN
-            const int field = static_cast<int>(m >> 23);
-            byte = m >= 0x7F800000u ? 255u : static_cast<uint32_t>(max(field - 2, 0));
-            scale = power_of_two(static_cast<int>(byte) - 127);
-            inv = power_of_two(127 - static_cast<int>(byte));
-            if (byte == 255u) inv = 0.0f;
+            byte = m >= 0x7F800000u ? 255u : static_cast<uint32_t>(max(static_cast<int>(m >> 23) - 2, 0));
+            scale = 0.0f;
+            inv = byte == 255u ? 0.0f : power_of_two(127 - static_cast<int>(byte));
         } else {
             byte = finite ? e4m3_byte(__fdiv_rn(__uint_as_float(m), six_g)) : 0u;
             scale = e4m3_value(byte) * g;
             inv = byte != 0u ? __frcp_rn(scale) : 0.0f;
         }
-        if (!live) continue;
+        if (!live) return;
         float q[kUnit];
+        unit.values(q);
 #pragma unroll
-        for (int e = 0; e < kUnit; ++e) q[e] = MX ? v[e] * inv : quotient(v[e], scale, inv);
-        const uint2 packed = inv != 0.0f ? make_uint2(codes8(q), codes8(q + 8)) : make_uint2(0u, 0u);
-        if (u * 8 < ld) *reinterpret_cast<uint2*>(crow + u * 8) = packed;
-        if (MX) {
-            if ((u & 1) == 0) stile[(u >> 3) * 512 + ((u >> 1) & 3)] = static_cast<uint8_t>(byte);
-        } else {
-            stile[(u >> 2) * 512 + (u & 3)] = static_cast<uint8_t>(byte);
+        for (int e = 0; e < kUnit; e += 2) {
+            if constexpr (MX) {
+                q[e] *= inv;
+                q[e + 1] *= inv;
+            } else {
+                quotients(q[e], q[e + 1], scale, inv);
+            }
         }
+        const uint2 packed = inv != 0.0f ? make_uint2(codes8(q), codes8(q + 8)) : make_uint2(0u, 0u);
+        if (static_cast<int64_t>(u) * 8 < ld) *reinterpret_cast<uint2*>(crow + static_cast<int64_t>(u) * 8) = packed;
+        if (MX) {
+            if ((u & 1) == 0) stile[static_cast<int64_t>(u >> 3) * 512 + ((u >> 1) & 3)] = static_cast<uint8_t>(byte);
+        } else {
+            stile[static_cast<int64_t>(u >> 2) * 512 + (u & 3)] = static_cast<uint8_t>(byte);
+        }
+    };
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h) {
+        const int u = static_cast<int>(threadIdx.x) + h * threads;
+        if (h * threads < units) pack(held[h], u, u < units);
+    }
+    for (int u0 = kHeld * threads; u0 < units; u0 += threads) {
+        const int u = u0 + static_cast<int>(threadIdx.x);
+        Unit<T> v;
+        if (u < units) v.load(row, static_cast<int64_t>(u) * kUnit, K, vector != 0);
+        pack(v, u, u < units);
     }
 }
 
@@ -248,7 +277,9 @@ int launch_quantize(const void* x, int64_t rows, int64_t K, int64_t ldx, int for
                     cudaStream_t stream) {
     const int vector = (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && (rows == 1 || ldx * sizeof(T) % 16 == 0);
     const int64_t units = (K + 255) / 256 * 16;
-    const int threads = static_cast<int>(std::min<int64_t>(kMaxThreads, (units + 31) / 32 * 32));
+    // two units a thread, or one where the rows do not fill the GPU
+    const int64_t wanted = rows > 4 * sm_count() ? (units + 1) / 2 : units;
+    const int threads = static_cast<int>(std::min<int64_t>(kMaxThreads, (wanted + 31) / 32 * 32));
     const T* p = static_cast<const T*>(x);
     if (format == BSI_FP4_MX)
         fp4_quantize_kernel<T, true><<<static_cast<unsigned>(rows), threads, 0, stream>>>(p, K, ldx, vector, codes, ld, scales, row_scale);
