@@ -9,8 +9,9 @@
 //
 //   warp 0     TMA producer: per k-block of 256 elements one box of weights (128 x 128 B), one of tokens (BN x 128 B), both 128-byte
 //              swizzled, and their scales as they lie in memory (512 bytes for 128 rows x 4 scales, whole tiles)
-//   warp 1     MMA issuer: tcgen05.cp of the block's scales into TMEM (two sets in turn), 4 MMAs of K = 64
+//   warp 1     MMA issuer: 4 MMAs of K = 64
 //   warps 2-5  epilogue
+//   warps 6-9  the block's scales from shared memory into TMEM, a set of columns for every stage of the operand ring
 // Where the tiles leave SMs idle, a cluster of 2, 4 or 8 CTAs shares a tile, each with a part of K; the parts' float32 sums meet in
 // shared memory and are added in the parts' order, each CTA for its share of the tokens.
 // Every wait is bounded: on a timeout the role records its site in the status word, raises the CTA's abort flag, what is under way is
@@ -42,7 +43,7 @@ namespace {
 
 constexpr int kRowBytes = 128;         // bytes of a k-block in a row: 256 elements
 constexpr int kTileM = 128;
-constexpr int kThreads = 192;
+constexpr int kThreads = 320;
 constexpr int kScaleTile = 512;        // 128 rows x 4 scales
 constexpr long long kWaitCycles = 500000000ll;    // about 0.25 s; real waits are microseconds
 constexpr int kSiteBase = 128;         // of the status word: sites 129 and up are this kernel's
@@ -59,11 +60,11 @@ struct Cfg {
     static constexpr int kPerSm = BN <= 64 ? 2 : 1;
     static constexpr int kBudget = (kPerSm == 2 ? 113 : 226) * 1024 - 2048;
     static constexpr int kStages = kBudget / kStageBytes > 8 ? 8 : kBudget / kStageBytes;
-    static constexpr int kSmem = kStages * kStageBytes + (2 * kStages + 2) * 8 + 32 + BN * 4 + 1024;
-    // TMEM: the accumulator, then two sets of scales (4 columns for each tile of 512 bytes)
+    static constexpr int kSmem = kStages * kStageBytes + (3 * kStages + 2) * 8 + 32 + BN * 4 + 1024;
+    // TMEM: the accumulator, then a set of scales for each stage (4 columns for each tile of 512 bytes)
     static constexpr int kScaleCols = 4 * kGroups * 2;
     static constexpr int kScale0 = BN < 32 ? 32 : BN;
-    static constexpr int kNeed = kScale0 + 2 * kScaleCols;
+    static constexpr int kNeed = kScale0 + kStages * kScaleCols;
     static constexpr int kTmemCols = kNeed <= 128 ? 128 : (kNeed <= 256 ? 256 : 512);
     static_assert(kStageBytes % 1024 == 0 && kStages >= 3 && kNeed <= 512 && kPerSm * kTmemCols <= 512, "does not fit");
     static_assert(BN * kTileM * 4 <= kStages * kStageBytes, "the parts' sums meet in the operand ring");
@@ -108,13 +109,52 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                  : "memory");
 }
 
-// 512 bytes of scales: 32 rows of 16 bytes, no swizzle, 8-row groups 128 bytes apart.
-__device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
-    return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128u >> 4) << 32) | (1ull << 46);
+template <int N>
+__device__ __forceinline__ void tmem_store(uint32_t taddr, const uint32_t* r) {
+    if constexpr (N >= 32) {
+        asm volatile(
+            "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+            "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+            ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+              "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+              "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+            : "memory");
+        if constexpr (N > 32) tmem_store<N - 32>(taddr + 32, r + 32);
+    } else if constexpr (N >= 16) {
+        asm volatile(
+            "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+            ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+              "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+            : "memory");
+        if constexpr (N > 16) tmem_store<N - 16>(taddr + 16, r + 16);
+    } else {
+        static_assert(N == 8, "columns in multiples of 8");
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                     ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+    }
 }
 
-__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+// One warp's share of a k-block's scales into TMEM: GROUPS tiles of 512 bytes of the weights, then GROUPS x NT of the tokens, group by
+// group. A tile is 32 lanes of 16 bytes, four columns; every quarter of TMEM's lanes holds the same, so each of four warps writes all.
+// (tcgen05.cp, which copies a tile into all quarters by itself, stands between the MMAs: 60 to 100 cycles for each tile, and 12 of them
+// beside the 512 cycles of a k-block's MMAs held 8192 x 4096 -> 16384 nvfp4 at 3.0 PFLOP/s where without them it ran at 5.0.)
+template <int GROUPS, int NT>
+__device__ __forceinline__ void scales_to_tmem(uint32_t tmem, const uint8_t* tiles) {
+    constexpr int kTiles = GROUPS * (1 + NT);
+    const int lane = threadIdx.x & 31;
+    uint32_t r[4 * kTiles];
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) {
+        const int b = j - GROUPS;
+        const int tile = j < GROUPS ? j : GROUPS + (b % NT) * GROUPS + b / NT;      // tokens' tiles lie row tile by row tile
+        const uint4 u = *reinterpret_cast<const uint4*>(tiles + tile * kScaleTile + lane * 16);
+        r[4 * j] = u.x;
+        r[4 * j + 1] = u.y;
+        r[4 * j + 2] = u.z;
+        r[4 * j + 3] = u.w;
+    }
+    tmem_store<4 * kTiles>(tmem, r);
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
 // e2m1 (1) at bits 7 and 10, N >> 3 at 17, e8m0 scales (1) at 23, M >> 7 at 27; which of a word's scales: bits 4 and 29.
@@ -178,14 +218,15 @@ __global__ void __launch_bounds__(kThreads) fp4_linear_kernel(const __grid_const
     constexpr int kStages = C::kStages;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * C::kStageBytes);      // full[], empty[], done, drain
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 2);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * C::kStageBytes);      // full[], empty[], scaled[], done, drained
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * kStages + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float* token_scale = reinterpret_cast<float*>(tmem_slot + 4);      // BN
     const uint32_t base = smem_u32(smem), bar0 = smem_u32(bars);
     auto full = [&](int s) { return bar0 + 8u * s; };
     auto empty = [&](int s) { return bar0 + 8u * (kStages + s); };
-    const uint32_t done = bar0 + 8u * (2 * kStages), drained = done + 8u;
+    auto scaled = [&](int s) { return bar0 + 8u * (2 * kStages + s); };
+    const uint32_t done = bar0 + 8u * (3 * kStages), drained = done + 8u;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int parts = static_cast<int>(cluster_size()), part = static_cast<int>(cluster_rank());
@@ -200,6 +241,7 @@ __global__ void __launch_bounds__(kThreads) fp4_linear_kernel(const __grid_const
         for (int s = 0; s < kStages; ++s) {
             mbar_init(full(s), 1);
             mbar_init(empty(s), 1);
+            mbar_init(scaled(s), 4);
         }
         mbar_init(done, 1);
         mbar_init(drained, 1);
@@ -256,21 +298,14 @@ __global__ void __launch_bounds__(kThreads) fp4_linear_kernel(const __grid_const
             bool ok = true;
             for (int i = 0; i < count; ++i) {
                 const int s = i % kStages;
-                if (!wait_for(full(s), static_cast<uint32_t>(i / kStages) & 1u, abort_flag, 2)) {
+                // the warps that write the scales have waited for the block
+                if (!wait_for(scaled(s), static_cast<uint32_t>(i / kStages) & 1u, abort_flag, 2)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
                 const uint32_t wa = base + s * C::kStageBytes, xa = wa + C::kWBytes;
-                const uint32_t sa = xa + C::kXBytes, sb = sa + C::kWScale;
-                // a set of columns is written again only two blocks later; copies and MMAs of one thread run in order
-                const uint32_t cols = tmem + C::kScale0 + (i & 1) * C::kScaleCols;
-                const uint32_t ca = cols, cb = cols + 4 * C::kGroups;
-#pragma unroll
-                for (int g = 0; g < C::kGroups; ++g) {
-                    copy_scales(ca + 4 * g, scale_desc(sa + g * kScaleTile));
-                    copy_scales(cb + 4 * g, scale_desc(sb + g * kScaleTile));
-                }
+                const uint32_t ca = tmem + C::kScale0 + s * C::kScaleCols, cb = ca + 4 * C::kGroups;
                 const uint64_t da = umma_desc(wa), db = umma_desc(xa);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -287,6 +322,18 @@ __global__ void __launch_bounds__(kThreads) fp4_linear_kernel(const __grid_const
                 drain(drained, 0);
             }
         }
+    } else if (warp >= 6) {
+        // A stage was loaded again only behind the MMAs that read its last scales, so its columns are free when it is full
+        const uint32_t cols = tmem + C::kScale0 + (static_cast<uint32_t>(warp & 3) << 21);      // its quarter: 32 lanes, at bit 16
+        for (int i = 0; i < count; ++i) {
+            const int s = i % kStages;
+            if (!__all_sync(0xFFFFFFFFu, wait_for(full(s), static_cast<uint32_t>(i / kStages) & 1u, abort_flag, 3))) break;
+            tc_fence_after();
+            scales_to_tmem<C::kGroups, 1>(cols + s * C::kScaleCols, smem + s * C::kStageBytes + C::kWBytes + C::kXBytes);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(scaled(s));
+        }
     }
     __syncwarp();
 
@@ -294,7 +341,7 @@ __global__ void __launch_bounds__(kThreads) fp4_linear_kernel(const __grid_const
     const int quad = warp & 3;
     const int feature = quad * 32 + lane;
     const int n = n0 + feature;
-    const bool epi = warp >= 2;
+    const bool epi = warp >= 2 && warp < 6;
     bool ok = true;
     float* sums = reinterpret_cast<float*>(smem);
     OutT* y = static_cast<OutT*>(a.y);
@@ -305,9 +352,9 @@ __global__ void __launch_bounds__(kThreads) fp4_linear_kernel(const __grid_const
             if (a.bias != nullptr) bias = a.bias[n];
         }
         if (a.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
-        for (int c = threadIdx.x - 64; c < BN; c += kThreads - 64) token_scale[c] = a.x_row != nullptr && c < a.M ? *behind_wait(a.x_row + c) : 1.0f;
+        for (int c = threadIdx.x - 64; c < BN; c += 128) token_scale[c] = a.x_row != nullptr && c < a.M ? *behind_wait(a.x_row + c) : 1.0f;
         asm volatile("bar.sync 1, 128;" ::: "memory");       // the four epilogue warps
-        ok = __all_sync(0xFFFFFFFFu, wait_for(done, 0, abort_flag, 3));
+        ok = __all_sync(0xFFFFFFFFu, wait_for(done, 0, abort_flag, 4));
         tc_fence_after();
     }
     auto store = [&](float v, int c) {
@@ -356,10 +403,15 @@ __global__ void __launch_bounds__(kThreads) fp4_linear_kernel(const __grid_const
 // MMAs at BN = 256; a CTA by itself with a tile of 128 x 256 would load 54 KB, and the way from L2 to an SM carries about 64 bytes a cycle.
 // Persistent: pairs walk over the tiles, loads run ahead into the next one, and the epilogue takes a finished accumulator into registers
 // in one go (8 warps, BN / 2 columns each), hands TMEM back and stores while the next tile's MMAs run.
-//   warp 0     TMA producer (both CTAs; every load signals the leader's barrier)
-//   warp 1     TMEM; MMA issuer (leader)
-//   warps 4-11 epilogue (both CTAs)
-constexpr int kPairThreads = 384;
+//   warp 0      TMA producer (both CTAs; operands signal the leader's barrier, a CTA's scales one of its own)
+//   warp 1      TMEM; MMA issuer (leader)
+//   warps 4-11  epilogue (both CTAs)
+//   warps 12-15 each block's scales into TMEM, a set of columns for every stage (both CTAs)
+// (Loads and MMAs issued by the scales' warps between blocks: the loads go out late, 3.4 PFLOP/s.)
+constexpr int kPairThreads = 512;
+constexpr int kPairRegsLow = 72, kPairRegsHigh = 184;       // an epilogue thread holds 128 sums
+// setmaxnreg.inc draws only on what the CTA was launched with
+static_assert(2 * 128 * kPairRegsLow + 2 * 128 * kPairRegsHigh <= kPairThreads * (65536 / kPairThreads / 8 * 8), "more registers than the CTA has");
 
 template <int BN, bool MX>
 struct PairCfg {
@@ -370,13 +422,14 @@ struct PairCfg {
     static constexpr int kWScale = kGroups * kScaleTile;
     static constexpr int kXScale = kNTiles * kGroups * kScaleTile;
     static constexpr int kStageBytes = kWBytes + kXBytes + kWScale + kXScale;
-    static constexpr int kFixed = 8 * (BN / 2) * 4 + 256 + 1024;      // token factors of the 8 epilogue warps, barriers and slots, alignment
+    static constexpr int kFixed = 8 * (BN / 2) * 4 + 512 + 1024;      // token factors of the 8 epilogue warps, barriers and slots, alignment
     static constexpr int kFit = (232448 - kFixed) / kStageBytes;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
     static constexpr int kSmem = kStages * kStageBytes + kFixed;
     static constexpr int kScaleCols = 4 * kGroups * (1 + kNTiles);
     static constexpr int kTmemCols = 512;
-    static_assert(kStageBytes % 1024 == 0 && kStages >= 4 && BN + 2 * kScaleCols <= kTmemCols && (2 * kStages + 3) * 8 + 16 <= 256, "does not fit");
+    static constexpr int kOperandBytes = kWBytes + kXBytes, kScaleBytes = kWScale + kXScale;
+    static_assert(kStageBytes % 1024 == 0 && kStages >= 4 && BN + kStages * kScaleCols <= kTmemCols && (4 * kStages + 3) * 8 + 16 <= 512, "does not fit");
 };
 
 __device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
@@ -388,10 +441,6 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
     asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(leader_bar)
                  : "memory");
-}
-// Each CTA's scales from its own shared memory into its own TMEM.
-__device__ __forceinline__ void copy_scales_pair(uint32_t tmem, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
 template <bool MX>
 __device__ __forceinline__ void umma_fp4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
@@ -459,14 +508,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     constexpr int kCols = BN / 2;        // columns of an epilogue warp
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * C::kStageBytes);      // full[], empty[], tfull, tempty, drained
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 3);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * C::kStageBytes);      // full[], empty[], loaded[], scaled[], tfull, tempty, drained
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 * kStages + 3);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    float* token_scale = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);      // [8][kCols]
+    float* token_scale = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 512);      // [8][kCols]
     const uint32_t base = smem_u32(smem), bar0 = smem_u32(bars);
     auto full = [&](int s) { return bar0 + 8u * s; };
     auto empty = [&](int s) { return bar0 + 8u * (kStages + s); };
-    const uint32_t tfull = bar0 + 8u * (2 * kStages), tempty = tfull + 8u, drained = tfull + 16u;
+    auto loaded = [&](int s) { return bar0 + 8u * (2 * kStages + s); };      // a CTA's own scales
+    auto scaled = [&](int s) { return bar0 + 8u * (3 * kStages + s); };      // the leader's: both CTAs' scales are in TMEM
+    const uint32_t tfull = bar0 + 8u * (4 * kStages), tempty = tfull + 8u, drained = tfull + 16u;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
@@ -477,6 +528,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         for (int s = 0; s < kStages; ++s) {
             mbar_init(full(s), 1);
             mbar_init(empty(s), 1);
+            mbar_init(loaded(s), 1);
+            mbar_init(scaled(s), 8);
         }
         mbar_init(tfull, 1);
         mbar_init(tempty, 16);       // the epilogue warps of both CTAs, at the leader's
@@ -495,90 +548,98 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0) {
-        if (lane == 0) {
+    const int64_t total = first < a.tiles ? static_cast<int64_t>((a.tiles - 1 - first) / step + 1) * a.blocks : 0;
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairRegsLow));
+        if (warp == 0 && lane == 0) {
             if (a.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
-            int s = 0, issued = 0;
+            int64_t issued = 0;
+            int s = 0, kb = 0, tile = first;
             uint32_t phase = 0;
-            bool ok = true;
-            for (int t = first; t < a.tiles && ok; t += step) {
-                const int n0 = t % a.tiles_n * 256, m0 = t / a.tiles_n * BN;
-                for (int kb = 0; kb < a.blocks; ++kb) {
-                    if (!wait(empty(s), phase ^ 1u, 1)) {
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t dst = base + s * C::kStageBytes, bar = in_cta(full(s), 0);
-                    if (rank == 0) mbar_expect_tx(full(s), 2 * C::kStageBytes);
-                    tma_load_pair(dst, &map_w, kb * kRowBytes, n0 + static_cast<int>(rank) * 128, bar);
-                    tma_load_pair(dst + C::kWBytes, &map_x, kb * kRowBytes, m0 + static_cast<int>(rank) * (BN / 2), bar);
-                    // tiles of 512 bytes are the rows of the scales' maps; a row tile beyond the last reads as zeros
-                    const uint32_t sc = dst + C::kWBytes + C::kXBytes;
-                    tma_load_pair(sc, &map_ws, 0, ((n0 >> 7) + static_cast<int>(rank)) * a.blocks * C::kGroups + kb * C::kGroups, bar);
+            while (issued < total && wait(empty(s), phase ^ 1u, 1)) {
+                const int n0 = tile % a.tiles_n * 256, m0 = tile / a.tiles_n * BN;
+                const uint32_t dst = base + s * C::kStageBytes, bar = in_cta(full(s), 0), own = loaded(s);
+                if (rank == 0) mbar_expect_tx(full(s), 2 * C::kOperandBytes);
+                mbar_expect_tx(own, C::kScaleBytes);
+                // tiles of 512 bytes are the rows of the scales' maps; a row tile beyond the last reads as zeros
+                const uint32_t sc = dst + C::kOperandBytes;
+                tma_load_2d(sc, &map_ws, 0, ((n0 >> 7) + static_cast<int>(rank)) * a.blocks * C::kGroups + kb * C::kGroups, own);
 #pragma unroll
-                    for (int q = 0; q < C::kNTiles; ++q)
-                        tma_load_pair(sc + C::kWScale + q * C::kGroups * kScaleTile, &map_xs, 0, ((m0 >> 7) + q) * a.blocks * C::kGroups + kb * C::kGroups, bar);
-                    ++issued;
-                    if (++s == kStages) {
-                        s = 0;
-                        phase ^= 1u;
-                    }
+                for (int q = 0; q < C::kNTiles; ++q)
+                    tma_load_2d(sc + C::kWScale + q * C::kGroups * kScaleTile, &map_xs, 0, ((m0 >> 7) + q) * a.blocks * C::kGroups + kb * C::kGroups, own);
+                tma_load_pair(dst, &map_w, kb * kRowBytes, n0 + static_cast<int>(rank) * 128, bar);
+                tma_load_pair(dst + C::kWBytes, &map_x, kb * kRowBytes, m0 + static_cast<int>(rank) * (BN / 2), bar);
+                ++issued;
+                if (++kb == a.blocks) {
+                    kb = 0;
+                    tile += step;
+                }
+                if (++s == kStages) {
+                    s = 0;
+                    phase ^= 1u;
                 }
             }
-            if (!ok && rank == 0) {
-                // let what was issued land (bounded); the barriers that count are the leader's
-                for (int i = max(0, issued - kStages); i < issued; ++i) drain(full(i % kStages), static_cast<uint32_t>(i / kStages) & 1u);
+            if (issued < total) {
+                // let what was issued land (bounded); the operands' barriers that count are the leader's
+                for (int64_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i) {
+                    const int q = static_cast<int>(i % kStages);
+                    const uint32_t p = static_cast<uint32_t>(i / kStages) & 1u;
+                    if (rank == 0) drain(full(q), p);
+                    drain(loaded(q), p);
+                }
             }
-        }
-    } else if (warp == 1 && rank == 0) {
-        if (lane == 0) {
-            int s = 0, count = 0;
+        } else if (warp == 1 && lane == 0 && rank == 0) {
+            int s = 0, kb = 0;
             uint32_t phase = 0, tphase = 0;
-            bool ok = true;
-            for (int t = first; t < a.tiles && ok; t += step) {
-                if (!wait(tempty, tphase ^ 1u, 2)) {
-                    ok = false;
-                    break;
-                }
-                tphase ^= 1u;
+            int64_t i = 0;
+            for (; i < total; ++i) {
+                if (!((kb != 0 || wait(tempty, tphase ^ 1u, 2)) && wait(full(s), phase, 3) && wait(scaled(s), phase, 4))) break;
                 tc_fence_after();
-                for (int kb = 0; kb < a.blocks; ++kb) {
-                    if (!wait(full(s), phase, 3)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t wa = base + s * C::kStageBytes, xa = wa + C::kWBytes, sa = xa + C::kXBytes, sb = sa + C::kWScale;
-                    const uint32_t ca = tmem + BN + (count & 1) * C::kScaleCols, cb = ca + 4 * C::kGroups;
+                const uint32_t wa = base + s * C::kStageBytes, xa = wa + C::kWBytes;
+                const uint32_t ca = tmem + BN + s * C::kScaleCols, cb = ca + 4 * C::kGroups;
+                const uint64_t da = umma_desc(wa), db = umma_desc(xa);
 #pragma unroll
-                    for (int g = 0; g < C::kGroups; ++g) {
-                        copy_scales_pair(ca + 4 * g, scale_desc(sa + g * kScaleTile));
-#pragma unroll
-                        for (int q = 0; q < C::kNTiles; ++q)
-                            copy_scales_pair(cb + 4 * (g * C::kNTiles + q), scale_desc(sb + (q * C::kGroups + g) * kScaleTile));
-                    }
-                    const uint64_t da = umma_desc(wa), db = umma_desc(xa);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int g = MX ? k >> 1 : k;
-                        umma_fp4_pair<MX>(tmem, da + 2u * k, db + 2u * k, instruction_pair<MX>(BN, MX ? (k & 1) * 2 : 0), ca + 4 * g,
-                                          cb + 4 * g * C::kNTiles, (kb | k) != 0 ? 1u : 0u);
-                    }
-                    commit_pair(empty(s));
-                    ++count;
-                    if (++s == kStages) {
-                        s = 0;
-                        phase ^= 1u;
-                    }
+                for (int k = 0; k < 4; ++k) {
+                    const int g = MX ? k >> 1 : k;
+                    umma_fp4_pair<MX>(tmem, da + 2u * k, db + 2u * k, instruction_pair<MX>(BN, MX ? (k & 1) * 2 : 0), ca + 4 * g, cb + 4 * g * C::kNTiles,
+                                      (kb | k) != 0 ? 1u : 0u);
                 }
-                if (ok) commit_pair(tfull);
+                commit_pair(empty(s));
+                if (++kb == a.blocks) {
+                    commit_pair(tfull);
+                    kb = 0;
+                    tphase ^= 1u;
+                }
+                if (++s == kStages) {
+                    s = 0;
+                    phase ^= 1u;
+                }
             }
-            if (!ok) {
+            if (i < total) {
                 commit_pair(drained);
                 drain(drained, 0);
             }
         }
-    } else if (warp >= 4) {
+    } else if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairRegsLow));
+        const uint32_t cols = tmem + BN + (static_cast<uint32_t>(warp & 3) << 21);      // the warp's quarter of the lanes, at bit 16
+        int s = 0;
+        uint32_t phase = 0;
+        for (int64_t i = 0; i < total; ++i) {
+            // A stage was loaded again only behind the MMAs that read its last scales, so its columns are free when it is full
+            if (!__all_sync(0xFFFFFFFFu, wait(loaded(s), phase, 5))) break;
+            tc_fence_after();
+            scales_to_tmem<C::kGroups, C::kNTiles>(cols + s * C::kScaleCols, smem + s * C::kStageBytes + C::kOperandBytes);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(in_cta(scaled(s), 0)) : "memory");
+            if (++s == kStages) {
+                s = 0;
+                phase ^= 1u;
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairRegsHigh));
         const int quad = warp & 3, half = (warp - 4) >> 2;
         if (a.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
         const uint32_t leader_tempty = in_cta(tempty, 0);
@@ -592,7 +653,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             for (int c = lane; c < kCols; c += 32) scale[c] = a.x_row != nullptr && m + c < a.M ? *behind_wait(a.x_row + m + c) : 1.0f;
             const float gw = a.w_row != nullptr && n < a.N ? a.w_row[n] : 1.0f, bias = a.bias != nullptr && n < a.N ? a.bias[n] : 0.0f;
             __syncwarp();
-            if (!__all_sync(0xFFFFFFFFu, wait(tfull, phase, 4))) break;
+            if (!__all_sync(0xFFFFFFFFu, wait(tfull, phase, 6))) break;
             phase ^= 1u;
             tc_fence_after();
             int32_t v[kCols / 32][32];

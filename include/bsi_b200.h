@@ -507,7 +507,7 @@ int bsi_b200_fp4_dequantize(const uint8_t* codes, int64_t ld, const uint8_t* sca
  * scales on the tensor cores, float32 sums, one rounding to y_dtype. bias float32 [N] or NULL; activation BSI_ACT_*. row scales are
  * factors of any float32 value. behind_packer != 0: the launch right before this one on the stream is the
  * bsi_b200_fp4_quantize that writes x, and nothing that may still run writes w: w is then read while x is still being packed. A wait
- * that gives up shows in bsi_b200_device_status as 129 to 131. */
+ * that gives up shows in bsi_b200_device_status as 129 to 134. */
 int bsi_b200_fp4_linear(const uint8_t* x_codes, int64_t ldx, const uint8_t* x_scales, const float* x_row_scale,
                         const uint8_t* w_codes, int64_t ldw, const uint8_t* w_scales, const float* w_row_scale, const float* bias,
                         int64_t M, int64_t N, int64_t K, int format, void* y, int64_t ldy, int y_dtype, int activation, int behind_packer,
