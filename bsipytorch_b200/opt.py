@@ -23,6 +23,7 @@ from torch.overrides import _get_current_function_mode_stack
 from torch.utils._device import DeviceContext
 
 from .linear import BSIQuantizedLinear, _ops
+from .scoring import distillation_loss, token_logprobs
 
 
 @dataclass
@@ -197,6 +198,18 @@ class OPTForCausalLM(nn.Module):
         """Last-position argmax, the reference's accuracy statistic (benchmark_performance_bsi.py:209-212)."""
         hidden = self.model.decoder(input_ids)[:, -1, :]
         return self.lm_head(hidden).argmax(dim=-1)
+
+    @torch.no_grad()
+    def score(self, input_ids, top_k: int = 0):
+        """What the model gives every token after the first, [batch, length - 1]: scoring.TokenLogprobs, with the top_k alternatives
+        of each position. ranks < 1 and < 5 are the reference's top-1 and top-5 hits, at every position instead of the last."""
+        return token_logprobs(self(input_ids)[:, :-1], input_ids[:, 1:], top_k)
+
+    def distillation_loss(self, input_ids, ids, teacher, **options):
+        """scoring.distillation_loss of this model's next-token logits against a teacher's top entries at the same positions, such as
+        ``top_ids`` and ``top_logprobs`` of the dense model's ``score(input_ids, top_k)`` (with ``tail=True``). Gradients reach the
+        parameters that are still dense; quantised linears pass none on."""
+        return distillation_loss(self(input_ids)[:, :-1], ids, teacher, **options)
 
 
 @torch.no_grad()
