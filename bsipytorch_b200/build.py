@@ -101,7 +101,7 @@ def build_ext(verbose: bool = False) -> str:
 
     srcs = [os.path.join(CSRC, n) for n in EXT_SOURCES]
     stamp = os.path.join(OBJ, "bsi_ops.stamp")
-    want = _hash(srcs + [os.path.join(CSRC, "lm_ops.h"), os.path.join(ROOT, "include", "bsi_b200.h")], torch.__version__ + EXT_SUFFIX)
+    want = _hash(srcs + [os.path.join(CSRC, "lm_ops.h"), os.path.join(CSRC, "block.h"), os.path.join(ROOT, "include", "bsi_b200.h")], torch.__version__ + EXT_SUFFIX)
     if _stamp_ok(stamp, want, EXT):
         return EXT
     os.makedirs(OBJ, exist_ok=True)

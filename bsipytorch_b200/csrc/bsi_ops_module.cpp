@@ -36,6 +36,7 @@
 #include <vector>
 
 #include "bsi_b200.h"
+#include "block.h"
 #include "lm_ops.h"
 
 namespace py = pybind11;
@@ -264,31 +265,6 @@ uint64_t g_last_quantize_ns = 0, g_last_pack_ns = 0, g_last_total_ns = 0;
 at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, at::Device dev) {
     return at::detail::empty_cuda(sizes, type, dev, c10::nullopt);
 }
-
-// Tensors that live and die together on one allocation: 0.7 us of host time for each after the first saved. Every
-// tensor starts on a 256-byte boundary of the block.
-class Block {
-public:
-    Block(int64_t bytes, at::Device dev)
-        : storage_(c10::Storage::use_byte_size_t{}, static_cast<size_t>(bytes), c10::cuda::CUDACachingAllocator::get()->allocate(static_cast<size_t>(bytes)),
-                   c10::cuda::CUDACachingAllocator::get(), /*resizable=*/false) {
-        TORCH_INTERNAL_ASSERT(storage_.device() == dev);
-    }
-    static int64_t room(int64_t bytes) { return (bytes + 255) / 256 * 256; }
-    at::Tensor take(at::IntArrayRef sizes, at::ScalarType type) {
-        at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(storage_), c10::DispatchKeySet(c10::DispatchKey::CUDA),
-                                                                c10::scalarTypeToTypeMeta(type));
-        t.unsafeGetTensorImpl()->set_storage_offset(used_ / static_cast<int64_t>(c10::elementSize(type)));
-        t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
-        used_ += room(static_cast<int64_t>(t.nbytes()));
-        TORCH_INTERNAL_ASSERT(used_ <= static_cast<int64_t>(storage_.nbytes()));
-        return t;
-    }
-
-private:
-    c10::Storage storage_;
-    int64_t used_ = 0;
-};
 
 // Quantise + pack `x` ([rows, d], f32/f16/bf16, CPU or CUDA) in one kernel.
 // lean = true skips the bit slices and slice weights (only the int8 image and the scales are

@@ -27,7 +27,6 @@ constexpr int kUnit = 16;            // elements of a thread at a time
 constexpr int kHeld = 2;             // units that a thread keeps between the search for the row's maximum and the rounding
 constexpr int kMaxThreads = 512;
 
-__device__ __forceinline__ float widen(float v) { return v; }
 __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
 __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
 
@@ -219,34 +218,35 @@ __global__ void __launch_bounds__(kMaxThreads, sizeof(T) == 4 ? 2 : 3)
     }
 }
 
+// A thread writes 16 bytes at a time, a warp 512 in a row; a row a CTA. What bounds it is the output's bytes.
 template <typename T, bool MX>
 __global__ void __launch_bounds__(256) fp4_dequantize_kernel(const uint8_t* __restrict__ codes, int64_t ld, const uint8_t* __restrict__ scales,
-                                                             const float* __restrict__ row_scale, int64_t rows, int64_t K, T* __restrict__ out, int64_t ldo,
-                                                             int vector) {
-    const int64_t units = (K + kUnit - 1) / kUnit;
+                                                             const float* __restrict__ row_scale, int64_t K, T* __restrict__ out, int64_t ldo, int vector) {
+    constexpr int kVec = 16 / sizeof(T);         // 4 or 8 elements, 2 or 4 bytes of codes, all of one block
+    const uint32_t r = blockIdx.x;
     const int64_t groups = (K + 255) / 256 * (MX ? 2 : 4);
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * units; i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t r = i / units, u = i % units;
-        const uint2 packed = *reinterpret_cast<const uint2*>(codes + r * ld + u * 8);
-        const int64_t block = MX ? u >> 1 : u;
-        const uint32_t byte = scales[((r / 128) * groups + (block >> 2)) * 512 + (r % 32) * 16 + (r % 128) / 32 * 4 + (block & 3)];
-        const float scale = MX ? (byte == 255u ? __uint_as_float(0x7FC00000u) : power_of_two(static_cast<int>(byte) - 127))
-                               : e4m3_value(byte) * row_scale[r];
-        float v[kUnit];
-        e2m1_values(packed.x, v);
-        e2m1_values(packed.y, v + 8);
-        alignas(16) T y[kUnit];
+    const uint8_t* crow = codes + r * ld;
+    const uint8_t* stile = scales + (r / 128) * groups * 512 + (r % 32) * 16 + (r % 128) / 32 * 4;
+    const float g = MX ? 1.0f : row_scale[r];
+    T* dst = out + r * ldo;
+    const int pieces = static_cast<int>((K + kVec - 1) / kVec);
+    for (int i = threadIdx.x; i < pieces; i += 256) {
+        const int block = i * kVec / (MX ? 32 : 16);
+        const uint32_t byte = stile[static_cast<int64_t>(block >> 2) * 512 + (block & 3)];
+        const float scale = MX ? (byte == 255u ? __uint_as_float(0x7FC00000u) : power_of_two(static_cast<int>(byte) - 127)) : e4m3_value(byte) * g;
+        // always all eight codes of a word: with the upper half of its bytes unread, the conversions of the lower came out as zeros
+        float v[8];
+        e2m1_values(reinterpret_cast<const uint32_t*>(crow)[i * kVec / 8], v);
+        alignas(16) T y[kVec];
 #pragma unroll
-        for (int e = 0; e < kUnit; ++e) y[e] = static_cast<T>(v[e] * scale);
-        T* dst = out + r * ldo + u * kUnit;
-        if (vector && (u + 1) * kUnit <= K) {
-#pragma unroll
-            for (int b = 0; b < static_cast<int>(kUnit * sizeof(T) / 16); ++b)
-                reinterpret_cast<uint4*>(dst)[b] = reinterpret_cast<const uint4*>(y)[b];
+        for (int e = 0; e < kVec; ++e) y[e] = static_cast<T>((kVec == 4 && (i & 1) != 0 ? v[(e + 4) % 8] : v[e]) * scale);
+        const int64_t c = static_cast<int64_t>(i) * kVec;
+        if (vector && c + kVec <= K) {
+            *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(y);
         } else {
 #pragma unroll
-            for (int e = 0; e < kUnit; ++e)
-                if (u * kUnit + e < K) dst[e] = y[e];
+            for (int e = 0; e < kVec; ++e)
+                if (c + e < K) dst[c + e] = y[e];
         }
     }
 }
@@ -292,13 +292,12 @@ template <typename T>
 int launch_dequantize(const uint8_t* codes, int64_t ld, const uint8_t* scales, const float* row_scale, int64_t rows, int64_t K, int format, void* out,
                       int64_t ldo, cudaStream_t stream) {
     const int vector = (reinterpret_cast<uintptr_t>(out) & 15u) == 0 && (rows == 1 || ldo * sizeof(T) % 16 == 0);
-    const int64_t units = rows * ((K + kUnit - 1) / kUnit);
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((units + 255) / 256, 1ll << 30));
+    const unsigned grid = static_cast<unsigned>(rows);
     T* p = static_cast<T*>(out);
     if (format == BSI_FP4_MX)
-        fp4_dequantize_kernel<T, true><<<grid, 256, 0, stream>>>(codes, ld, scales, row_scale, rows, K, p, ldo, vector);
+        fp4_dequantize_kernel<T, true><<<grid, 256, 0, stream>>>(codes, ld, scales, row_scale, K, p, ldo, vector);
     else
-        fp4_dequantize_kernel<T, false><<<grid, 256, 0, stream>>>(codes, ld, scales, row_scale, rows, K, p, ldo, vector);
+        fp4_dequantize_kernel<T, false><<<grid, 256, 0, stream>>>(codes, ld, scales, row_scale, K, p, ldo, vector);
     return check_launch("fp4_dequantize launch");
 }
 

@@ -10,6 +10,7 @@
 
 #include <vector>
 
+#include "block.h"
 #include "bsi_b200.h"
 
 namespace py = pybind11;
@@ -36,6 +37,9 @@ int dtype_code(const at::Tensor& t, const char* what) {
         default: TORCH_CHECK(false, what, " must be float32, float16 or bfloat16, got ", t.scalar_type());
     }
 }
+
+// A plain tensor that wants no gradients needs no detached alias.
+at::Tensor plain(const at::Tensor& t) { return t.requires_grad() ? t.detach() : t; }
 
 void on_device(const at::Tensor& t, at::Device dev, const char* what) {
     TORCH_CHECK(t.device() == dev, what, " must live on the logits' device ", dev, ", got ", t.device());
@@ -79,7 +83,7 @@ struct Logits {
     int code;
     std::vector<int64_t> lead;
 
-    explicit Logits(const at::Tensor& given) : t(given.detach()) {
+    explicit Logits(const at::Tensor& given) : t(plain(given)) {
         TORCH_CHECK(t.is_cuda(), "logits must be a CUDA tensor: there is no CPU path");
         TORCH_CHECK(t.dim() >= 1 && t.size(-1) >= 1, "logits must be [..., vocabulary]");
         code = dtype_code(t, "logits");
@@ -99,7 +103,7 @@ py::tuple token_logprobs(const torch::Tensor& logits, const OptTensor& tokens, i
     at::Tensor ids;
     bsi_row_plan ids_at{0, 0, 0};
     if (tokens.has_value()) {
-        ids = tokens->detach();
+        ids = plain(*tokens);
         on_device(ids, z.t.device(), "tokens");
         TORCH_CHECK(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt, "tokens must be int64 or int32, got ", ids.scalar_type());
         TORCH_CHECK(ids.sizes() == at::IntArrayRef(z.lead), "tokens must have the logits' leading shape ", at::IntArrayRef(z.lead), ", got ", ids.sizes());
@@ -107,8 +111,10 @@ py::tuple token_logprobs(const torch::Tensor& logits, const OptTensor& tokens, i
         if (z.rows > 0) ids_at = plan_rows(ids, 0);
     }
     const at::Device dev = z.t.device();
-    at::Tensor logprobs = fresh(z.lead, at::kFloat, dev), ranks = fresh(z.lead, at::kLong, dev), entropy = fresh(z.lead, at::kFloat, dev);
-    at::Tensor top = fresh(with_last(z.lead, top_k), at::kFloat, dev), top_ids = fresh(with_last(z.lead, top_k), at::kLong, dev);
+    Block block(Block::room(z.rows * 4) * 2 + Block::room(z.rows * 8) + Block::room(z.rows * top_k * 4) + Block::room(z.rows * top_k * 8) + 256, dev);
+    const std::vector<int64_t> with_top = with_last(z.lead, top_k);
+    at::Tensor logprobs = block.take(z.lead, at::kFloat), ranks = block.take(z.lead, at::kLong), entropy = block.take(z.lead, at::kFloat);
+    at::Tensor top = block.take(with_top, at::kFloat), top_ids = block.take(with_top, at::kLong);
     check_status(bsi_b200_token_logprobs(z.t.data_ptr(), z.code, z.rows, z.V, &z.plan, ids.defined() ? ids.data_ptr<int64_t>() : nullptr, &ids_at,
                                          static_cast<int>(top_k), logprobs.data_ptr<float>(), ranks.data_ptr<int64_t>(), entropy.data_ptr<float>(),
                                          top.data_ptr<float>(), top_ids.data_ptr<int64_t>(), current_stream()),
@@ -123,8 +129,8 @@ struct Teacher {
 
     Teacher(const Logits& z, const at::Tensor& given_ids, const at::Tensor& given, const OptTensor& w) {
         const at::Device dev = z.t.device();
-        ids = given_ids.detach();
-        values = given.detach();
+        ids = plain(given_ids);
+        values = plain(given);
         on_device(ids, dev, "ids");
         on_device(values, dev, "the teacher's values");
         TORCH_CHECK(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt, "ids must be int64 or int32, got ", ids.scalar_type());
@@ -133,13 +139,15 @@ struct Teacher {
                     "ids and the teacher's values must both be ", at::IntArrayRef(z.lead), " by entries, got ", ids.sizes(), " and ", values.sizes());
         TORCH_CHECK(ids.size(-1) >= 1 && ids.size(-1) <= 512, "1 to 512 teacher entries a row are taken, got ", ids.size(-1));
         K = static_cast<int>(ids.size(-1));
-        ids = ids.to(at::kLong).contiguous();
-        values = values.contiguous();
+        if (ids.scalar_type() != at::kLong) ids = ids.to(at::kLong);
+        if (!ids.is_contiguous()) ids = ids.contiguous();
+        if (!values.is_contiguous()) values = values.contiguous();
         if (w.has_value()) {
-            weights = w->detach();
+            weights = plain(*w);
             on_device(weights, dev, "weights");
             TORCH_CHECK(weights.sizes() == at::IntArrayRef(z.lead), "weights must have the logits' leading shape ", at::IntArrayRef(z.lead), ", got ", weights.sizes());
-            weights = weights.to(at::kFloat).contiguous();
+            if (weights.scalar_type() != at::kFloat) weights = weights.to(at::kFloat);
+            if (!weights.is_contiguous()) weights = weights.contiguous();
         }
     }
     const float* weight() const { return weights.defined() ? weights.data_ptr<float>() : nullptr; }
@@ -221,9 +229,11 @@ struct Fp4 {
 
     // Nothing but room.
     Fp4(int64_t r, int64_t k, int f, at::Device dev) : rows(r), K(k), format(f) {
-        codes = fresh({rows, (K + 31) / 32 * 16}, at::kByte, dev);
-        scales = fresh({bsi_b200_fp4_scale_bytes(rows, K, format)}, at::kByte, dev);
-        if (format == BSI_FP4_NV) row_scale = fresh({rows}, at::kFloat, dev);
+        const int64_t ld = (K + 31) / 32 * 16, tiles = bsi_b200_fp4_scale_bytes(rows, K, format);
+        Block block(Block::room(rows * ld) + Block::room(tiles) + Block::room(rows * 4) + 256, dev);
+        codes = block.take({rows, ld}, at::kByte);
+        scales = block.take({tiles}, at::kByte);
+        if (format == BSI_FP4_NV) row_scale = block.take({rows}, at::kFloat);
     }
     // A matrix that a caller holds.
     Fp4(const at::Tensor& c, const at::Tensor& s, const OptTensor& g, int64_t k, int f) : codes(c), scales(s), rows(c.size(0)), K(k), format(f) {
@@ -248,7 +258,7 @@ void quantize_into(const at::Tensor& x2d, Fp4& to) {
 }
 
 at::Tensor as_rows(const at::Tensor& given, const char* what) {
-    at::Tensor t = given.detach();
+    at::Tensor t = plain(given);
     TORCH_CHECK(t.is_cuda(), what, " must be a CUDA tensor: there is no CPU path");
     TORCH_CHECK(t.dim() >= 1 && t.size(-1) >= 1, what, " must be [..., features]");
     dtype_code(t, what);
@@ -281,7 +291,9 @@ at::Tensor fp4_dequantize(const torch::Tensor& codes, const torch::Tensor& scale
 at::Tensor bias_of(const OptTensor& bias, const Fp4& w) {
     if (!bias.has_value()) return at::Tensor();
     TORCH_CHECK(bias->device() == w.codes.device() && bias->numel() == w.rows, "one bias per output, on the weights' device");
-    return bias->detach().to(at::kFloat).contiguous();
+    at::Tensor b = plain(*bias);
+    if (b.scalar_type() != at::kFloat) b = b.to(at::kFloat);
+    return b.is_contiguous() ? b : b.contiguous();
 }
 
 at::Tensor product(const Fp4& x, const Fp4& w, const at::Tensor& bias, bool relu, at::ScalarType type, bool behind_packer) {
