@@ -35,10 +35,9 @@ using vocab::Span;
 using vocab::Stats;
 
 constexpr int kMaxTop = 128;            // alternatives of token_logprobs
-constexpr int kCandidates = 1024;       // entries at least as large as the bound of their time that a block keeps
-constexpr int kSorted = 64;             // above so many they are thinned out by the last bound before they are put in order
-constexpr int kPerSm = 3;               // CTAs of 256 threads with 80 registers
-constexpr int kStages = 2;              // chunks under way in each: 96 KB an SM, 6.2 TB/s where nothing but the statistics is computed
+constexpr int kCandidates = 1024;       // entries at least as large as the last bound that a block keeps
+constexpr int kPerSm = 4;               // CTAs of 256 threads with 64 registers: a row's end takes as long as a third of 100 KB, and others fill it
+constexpr int kStages = 2;              // chunks under way in each: 128 KB an SM
 constexpr int kMaxListed = 512;         // teacher entries per row
 static_assert(vocab::kMaxCluster * kMaxTop <= kCandidates, "CTA 0 gathers the others' lists where its candidates were");
 
@@ -48,11 +47,12 @@ static_assert(vocab::kMaxCluster * kMaxTop <= kCandidates, "CTA 0 gathers the ot
 // rank = #{z_j > z_t} + #{j < t, z_j = z_t}, top = the k largest, equal values by ascending index.
 //
 // The top k ride on the same pass. Every warp knows the j-th largest of its lanes' running maxima, j = ceil(k / 8); with B the t-th
-// largest of these over the 8 warps, t = ceil(k / j), at least k entries are >= B, so the k largest all are, and few others. The bound
-// is found behind the first chunk, which the threads still hold (one barrier), and again behind chunks 2, 4, 8, ... without one: any
-// bound of an earlier time is one. Entries that reach the bound of their time are kept (about k for each doubling of what was read), and put in order at the end by
-// counting for each one how many come before it. Reading a row again where a thread's maximum reaches the final bound costs a quarter of
-// the row from memory at k = 64 (633 x 128011 float32: 163 us).
+// largest of these over the 8 warps, t = ceil(k / j), at least k entries are >= B, so the k largest all are, and few others. It is
+// worked out behind chunks 1, 2, 4, 8, ... without any barrier, as a bound of an earlier time is one too; a thread only notes which of
+// its batches reached the bound of their time, a bit each. At the row's end the last bound is a tight one, and the few batches noted
+// are read again, out of L2, for the entries that reach it, which are put in order by counting for each one how many come before it.
+// (633 x 128011 float32, k = 64: keeping the entries themselves as the row goes by took 138 us, reading again all that a thread whose
+// maximum reaches the last bound had read, 163.)
 // Where more than kCandidates entries are kept (a row in ascending order, a constant one), the block selects by radix: four passes over
 // 8 bits each give the k-th value, one pass the larger entries, one in index order the equal ones. -inf is kept only where a row has
 // fewer than k other entries.
@@ -268,68 +268,63 @@ __global__ void __launch_bounds__(kThreads, kPerSm) score_kernel(const ScoreArgs
     const int mine = max(span.end() - span.begin(), 0);
     const int k = min(a.top, mine);
     const int pieces = span.whole_last() - span.whole_first();
-    // warps whose lanes all have a piece from the start vote; fewer than four of them: less than kCandidates entries in all, or few rounds
+    // warps whose lanes all have a piece from the start vote
     const int voters = max(1, min(kWarps, pieces / 32)), j = max(1, (k + voters - 1) / voters), t = (k + j - 1) / j;
     if (tid == 0) {
         sh.found = 0;
         sh.agreed_bound = 0;
     }
+    if (tid < kWarps) sh.bound[tid] = 0;       // no warp has one for this row yet
     me.set_bound(0);
     __syncthreads();       // the ring's barriers, the count, and nobody is at the row before
-    int round = 0;
-    auto agree = [&]() {       // a bound from what has been read so far
-        if ((round & (round + 1)) == 0) {
-            const uint32_t own = warp_bound(Piece<T>::place(me.run.m), j);
-            if (lane == 0) sh.bound[warp] = own;
-            if (round == 0) __syncthreads();
-            const uint32_t all = sh.agreed(voters, t);
-            if (lane == 0) atomicMax(&sh.agreed_bound, all);
-            __syncwarp();
-        }
-        me.set_bound(*static_cast<volatile uint32_t*>(&sh.agreed_bound));
-        ++round;
+    auto publish = [&]() {
+        const uint32_t own = warp_bound(Piece<T>::place(me.run.m), j);
+        if (lane == 0) sh.bound[warp] = own;
+        __syncwarp();
+        return sh.agreed(voters, t);
     };
-    for (int i = 0; i < pieces; i += kChunk) {
+    // bit: one batch, or as many as 64 bits have to share (rows of more than a megabyte a part)
+    const int share = (pieces + 64 * kChunk - 1) / (64 * kChunk);
+    unsigned long long noted = 0;
+    float first_largest = -CUDART_INF_F;
+    for (int i = 0, n = 0; i < pieces; i += kChunk, ++n) {
         const uint4* chunk = ring.arrive(place);
         const int v = span.whole_first() + i + tid;
+        float largest = -CUDART_INF_F;
         if (i + kChunk <= pieces) {
             uint4 u[kBatch];
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) u[b] = chunk[tid + b * kThreads];
-            const float largest = me.take(u, v);
-            if (top) {
-                agree();
-                me.keep(sh, span, u, v, largest, reinterpret_cast<const T*>(chunk + tid));
-            }
+            largest = me.take(u, v);
         } else {
             // the part's last pieces
-            for (int b = 0; i + b * kThreads < pieces; ++b) {
-                const bool in = i + b * kThreads + tid < pieces;
-                uint4 u[1];
-                float largest = -CUDART_INF_F;
-                if (in) {
-                    u[0] = chunk[tid + b * kThreads];
-                    largest = me.take(u, v + b * kThreads);
-                }
-                if (top) {
-                    __syncwarp();
-                    if (round == 0) agree();
-                    if (in) me.keep(sh, span, u, v + b * kThreads, largest, reinterpret_cast<const T*>(chunk + tid + b * kThreads));
-                }
+            for (int b = 0; i + b * kThreads + tid < pieces; ++b) {
+                const uint4 u[1] = {chunk[tid + b * kThreads]};
+                largest = vocab::max_nan(largest, me.take(u, v + b * kThreads));
             }
+            __syncwarp();
         }
         ring.release(place);
         ring.advance(place);
+        if (top) {
+            if (n == 0) first_largest = largest;
+            else if (!(largest < me.bound)) noted |= 1ull << (n / share);
+            if ((n & (n + 1)) == 0) {
+                const uint32_t all = publish();
+                if (lane == 0) atomicMax(&sh.agreed_bound, all);
+            }
+            me.set_bound(*static_cast<volatile uint32_t*>(&sh.agreed_bound));
+        }
     }
+    if (top) publish();
     T zt_next = Piece<T>::nan();
     if (wanted_next >= 0 && wanted_next < V) zt_next = (static_cast<const T*>(a.logits) + a.rows.at(r + step))[wanted_next];
     // the row's ends; -inf in the places that are not the row's, which a token at -inf would count on the left
     if ((tid == 0 && span.has_left()) || (tid == 32 && span.has_right())) {
         const int v = tid == 0 ? span.first : span.last - 1;
         const uint4 u[1] = {span.load_edge(v)};
-        const float largest = me.take(u, v);
+        me.take(u, v);
         if (span.element(v) < 0 && v < me.token_piece && Piece<T>::one(zt) == -CUDART_INF_F) me.ahead += span.element(v);
-        if (top) me.keep(sh, span, u, v, largest, row + span.element(v));
     }
 
     // the block's statistics
@@ -351,35 +346,37 @@ __global__ void __launch_bounds__(kThreads, kPerSm) score_kernel(const ScoreArgs
         }
     }
 
-    if (a.top > 0) {
+    if (top) {
+        me.set_bound(sh.agreed(voters, t));
+        if (!(first_largest < me.bound)) noted |= 1ull;
+        while (noted != 0ull) {
+            const int bit = __ffsll(static_cast<long long>(noted)) - 1;
+            noted &= noted - 1ull;
+            for (int n = bit * share; n < (bit + 1) * share && n * kChunk + tid < pieces; ++n) {
+                const int v = span.whole_first() + n * kChunk + tid;
+                uint4 u[kBatch];
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b)
+                    u[b] = v + b * kThreads < span.whole_last() ? span.grid[v + b * kThreads] : make_uint4(Piece<T>::kNone, Piece<T>::kNone, Piece<T>::kNone, Piece<T>::kNone);
+                me.keep(sh, span, u, v, Piece<T>::top(u), row + span.element(v));
+            }
+        }
+        if ((tid == 0 && span.has_left()) || (tid == 32 && span.has_right())) {
+            const int v = tid == 0 ? span.first : span.last - 1;
+            const uint4 u[1] = {span.load_edge(v)};
+            me.keep(sh, span, u, v, Piece<T>::top(u), row + span.element(v));
+        }
+        __syncthreads();
         int n = sh.found;
-        me.set_bound(sh.agreed_bound);
-        unsigned long long least = static_cast<unsigned long long>(vocab::ordered(me.bound)) << 32;
         if (n > kCandidates) {
             __syncthreads();      // everybody has read how many there were
             select_by_radix<T>(sh, row, span.begin(), span.end(), k);
             n = k;
-            least = 0;
         } else if (n < k) {
             // fewer entries than that are above -inf, and all of them are kept
             __syncthreads();
             take_equal<T>(sh, row, span.begin(), span.end(), vocab::ordered(-CUDART_INF_F), n, k - n);
             n = k;
-            least = 0;
-        }
-        if (n > kSorted) {
-            // those that the last bound leaves, in their buffer's front
-            unsigned long long mine_of[kCandidates / kThreads];
-#pragma unroll
-            for (int q = 0; q < kCandidates / kThreads; ++q) mine_of[q] = tid + q * kThreads < n ? sh.cand[tid + q * kThreads] : 0ull;
-            __syncthreads();
-            if (tid == 0) sh.found = 0;
-            __syncthreads();
-#pragma unroll
-            for (int q = 0; q < kCandidates / kThreads; ++q)
-                if (tid + q * kThreads < n && mine_of[q] >= least) sh.cand[atomicAdd(&sh.found, 1)] = mine_of[q];
-            __syncthreads();
-            n = sh.found;
         }
         for (int i = tid; i < n; i += kThreads) {
             const unsigned long long key = sh.cand[i];
@@ -447,25 +444,24 @@ __global__ void __launch_bounds__(kThreads, kPerSm) score_kernel(const ScoreArgs
     }
 }
 
-// CTAs per row and rows under way. As many CTAs as the GPU holds walk over the rows; a CTA's time for a row is about its bytes at 11 per
-// ns (a quarter of an SM's share of the memory's rate) and 3 us for what the row's end takes, which the other CTAs of the SM fill. The
-// number of parts for which the longest walk is shortest.
-constexpr double kSmRate = 42000.0;     // bytes per us of an SM's share of the memory's rate
-constexpr double kEnd = 6.0;            // us of a row's end, by which parts cost
+// CTAs per row and rows under way: as many CTAs as the GPU holds walk over the rows. An SM takes its share of them at its share of the
+// memory's rate, 42 bytes per ns, unless a CTA's own pace holds it up: 20 bytes per ns, and the end of a row, 4 us, or 8 where a cluster
+// has to join its parts. The number of parts for which that is shortest. (633 x 128011 float32: one part 70 us, two 117.)
 struct Walk {
     int parts;
     int64_t clusters;
 };
 Walk walk_over(int64_t rows, int64_t V, int esz, int least_parts, int per_sm) {
-    const int64_t slots = static_cast<int64_t>(per_sm) * sm_count();
+    const int64_t sms = sm_count();
     Walk best{0, 0};
     double least = 0.0;
     for (int parts = least_parts; parts <= vocab::kMaxCluster; parts *= 2) {
-        const int64_t clusters = std::min(rows, std::max<int64_t>(1, slots / parts));
-        const double cost = static_cast<double>((rows + clusters - 1) / clusters) * (static_cast<double>(V) * esz / parts * per_sm / kSmRate + kEnd);
+        const double bytes = static_cast<double>(V) * esz / parts, end = parts > 1 ? 8.0 : 4.0;
+        const int64_t mine = (rows * parts + sms - 1) / sms, rounds = (mine + per_sm - 1) / per_sm;       // of one SM
+        const double cost = std::max(static_cast<double>(mine) * bytes / 42000.0 + end, static_cast<double>(rounds) * (bytes / 20000.0 + end));
         if (best.parts == 0 || cost < least) {
             least = cost;
-            best = Walk{parts, clusters};
+            best = Walk{parts, std::min(rows, std::max<int64_t>(1, sms * per_sm / parts))};
         }
     }
     return best;
