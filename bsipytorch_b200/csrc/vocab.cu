@@ -515,7 +515,7 @@ int check_rows(const char* what, const void* logits, int dtype, int64_t rows, in
         set_error("%s: dtype must be a BSI_DTYPE_* code, got %d", what, dtype);
         return BSI_ERR_INVALID;
     }
-    if (rows < 0 || V < 1 || rows > kMaxRows || V > 0x7FFFFFFFll) {
+    if (rows < 0 || V < 1 || rows > kMaxRows || V > (1ll << 30)) {      // pieces' elements are counted in 32 bits
         set_error("%s: %lld rows of %lld logits", what, static_cast<long long>(rows), static_cast<long long>(V));
         return BSI_ERR_INVALID;
     }
@@ -581,6 +581,9 @@ struct DistillShared {
     vocab::Feed feed;
     Stats rest, listed;          // of this CTA's part of the row, read by the other CTAs
     float total_p;
+    long long raw_id[kMaxListed];      // as they lie in memory
+    float raw_t[kMaxListed];
+    uint32_t raw_z[kMaxListed];
     Entry entry[kMaxListed];
 };
 
@@ -590,20 +593,58 @@ __device__ __forceinline__ float teacher_value(const void* t, int dtype, int64_t
     return __bfloat162float(static_cast<const __nv_bfloat16*>(t)[i]);
 }
 
-// The row's entries with their probabilities and logits, by one warp (a few values per lane); the caller synchronises.
+// The row's entries with their probabilities and logits, by one warp in three steps. Each step's values come from memory while something
+// else goes on: ids and the teacher's values during the end of the row before, the logits that they name while the row streams.
+__device__ __forceinline__ void copy_async(void* dst, const void* src, bool eight) {
+    const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+    if (eight) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_done() {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+}
+
+__device__ __forceinline__ void ask_entries(DistillShared& sh, const DistillArgs& a, int64_t r) {
+    for (int k = threadIdx.x & 31; k < a.K; k += 32) {
+        copy_async(&sh.raw_id[k], a.ids + r * a.K + k, true);
+        // 16-bit values are read when they are used: there is no copy of two bytes
+        if (a.teacher_dtype == BSI_DTYPE_F32) copy_async(&sh.raw_t[k], static_cast<const float*>(a.teacher) + r * a.K + k, false);
+    }
+}
 template <typename T>
-__device__ void read_entries(DistillShared& sh, const DistillArgs& a, int64_t r, const T* row) {
+__device__ __forceinline__ void ask_logits(DistillShared& sh, const DistillArgs& a, const T* row) {
+    copies_done();
+    for (int k = threadIdx.x & 31; k < a.K; k += 32) {
+        const int64_t id = sh.raw_id[k];
+        const bool there = id >= 0 && id < a.V;
+        sh.entry[k].id = there ? static_cast<int>(id) : -1;
+        // the 4 bytes that hold it
+        if (there) copy_async(&sh.raw_z[k], reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(row + id) & ~uintptr_t(3)), false);
+    }
+}
+template <typename T>
+__device__ void finish_entries(DistillShared& sh, const DistillArgs& a, int64_t r, const T* row) {
     const int lane = threadIdx.x & 31;
     const float inv_t = 1.0f / a.temperature;
+    copies_done();
     float top = -CUDART_INF_F;
     for (int k = lane; k < a.K; k += 32) {
-        const int64_t id = a.ids[r * a.K + k];
-        const bool there = id >= 0 && id < a.V;
-        float t = there ? teacher_value(a.teacher, a.teacher_dtype, r * a.K + k) : -CUDART_INF_F;
+        const int id = sh.entry[k].id;
+        float t = -CUDART_INF_F, z = 0.0f;
+        if (id >= 0) {
+            t = a.teacher_dtype == BSI_DTYPE_F32 ? sh.raw_t[k] : teacher_value(a.teacher, a.teacher_dtype, r * a.K + k);
+            const uint32_t word = sh.raw_z[k];
+            if constexpr (sizeof(T) == 4) {
+                z = __uint_as_float(word);
+            } else {
+                const unsigned short half = static_cast<unsigned short>((reinterpret_cast<uintptr_t>(row + id) & 2u) ? word >> 16 : word & 0xFFFFu);
+                z = Piece<T>::one(*reinterpret_cast<const T*>(&half));
+            }
+        }
         if (!a.tail) t *= inv_t;
-        sh.entry[k].id = there ? static_cast<int>(id) : -1;
         sh.entry[k].logp = t;
-        sh.entry[k].z = there ? Piece<T>::one(row[id]) : 0.0f;
+        sh.entry[k].z = z;
         top = vocab::max_nan(top, t);
     }
     float norm = 0.0f;
@@ -758,6 +799,14 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const Distill
     uint32_t r = blockIdx.x / static_cast<unsigned>(parts);
     Ring<T> ring(data, bars, stages, &sh.feed, a.logits, a.rows, V, part, parts, a.weights, r, step, a.count, &g_vocab_status);
     typename Ring<T>::Place place{0, 0};
+    auto next_read = [&](uint32_t q) {       // the first row from q on that is read
+        while (q < a.count && a.weights != nullptr && a.weights[q] == 0.0f) q += step;
+        return q;
+    };
+    if (warp == kWarps - 1) {
+        const uint32_t q = next_read(r);
+        if (q < a.count) ask_entries(sh, a, q);
+    }
     for (; r < a.count; r += step) {
     const T* row = static_cast<const T*>(a.logits) + a.rows.at(r);
     const Span<T> span(row, V, part, parts);
@@ -776,8 +825,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const Distill
     }
     __syncthreads();      // nobody is at the row before
 
-    // The last warp reads the entries; with the tail off nobody waits for it before the row's end
-    if (warp == kWarps - 1) read_entries<T>(sh, a, r, row);
+    // The last warp has the entries
+    if (warp == kWarps - 1) ask_logits<T>(sh, a, row);
     const float c = vocab::kLog2e / a.temperature;
     const int bit0 = span.element(span.first);         // the part's bit 0; kVec bits for each piece
     const int lo = span.begin(), hi = span.end();
@@ -792,7 +841,6 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const Distill
     }
 
     vocab::Running<T, false> run;
-    __syncthreads();
     // a piece as the statistics see it: listed logits out where they are summed apart
     auto seen = [&](uint4& u, int v) {
         if (a.tail) {
@@ -840,6 +888,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const Distill
 
     Stats st = vocab::warp_merge(run.stats(c), c);
     if (lane == 0) sh.warp[warp] = st;
+    if (warp == kWarps - 1) {
+        finish_entries<T>(sh, a, r, row);
+        const uint32_t q = next_read(r + step);
+        if (q < a.count) ask_entries(sh, a, q);
+    }
     __syncthreads();
     Stats listed{-CUDART_INF_F, 0.0f, 0.0f};
     if (a.tail) {
@@ -931,7 +984,11 @@ __global__ void __launch_bounds__(kThreads, 4) distill_backward_kernel(const Dis
     const T* row = static_cast<const T*>(a.logits) + a.rows.at(r);
     const Span<T> span(row, static_cast<int>(a.V), static_cast<int>(blockIdx.x % parts), parts);
     const float4 saved = a.saved[r];
-    if (saved.w != 0.0f && threadIdx.x >= kThreads - 32) read_entries<T>(sh, a, r, row);
+    if (saved.w != 0.0f && threadIdx.x >= kThreads - 32) {
+        ask_entries(sh, a, r);
+        ask_logits<T>(sh, a, row);
+        finish_entries<T>(sh, a, r, row);
+    }
     const Gradient<T> g(a, r, span, saved, grad_scale(a, r));
     g.write_part(span);
     g.write_ends(span);
@@ -1028,6 +1085,10 @@ int check_distill(const char* what, const void* logits, int dtype, int64_t rows,
     }
     if (teacher_dtype != BSI_DTYPE_F32 && teacher_dtype != BSI_DTYPE_F16 && teacher_dtype != BSI_DTYPE_BF16) {
         set_error("%s: teacher dtype must be a BSI_DTYPE_* code, got %d", what, teacher_dtype);
+        return BSI_ERR_INVALID;
+    }
+    if (reinterpret_cast<uintptr_t>(ids) % 8 != 0 || reinterpret_cast<uintptr_t>(teacher) % (teacher_dtype == BSI_DTYPE_F32 ? 4 : 2) != 0) {
+        set_error("%s: misaligned ids or teacher", what);
         return BSI_ERR_INVALID;
     }
     if (!(temperature > 0.0f) || !(temperature <= 3.0e38f)) {

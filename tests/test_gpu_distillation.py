@@ -222,6 +222,46 @@ def test_same_bits_and_a_captured_step():
     assert all(torch.equal(p, q) for p, q in zip(fused, held))
 
 
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_a_captured_training_step(reduction):
+    """Forward and backward in one graph, on new logits at every replay, as a training loop that is launch-bound records them."""
+    z, ids, t, w = (x.cuda() for x in case(6, 3001, 12, torch.float16, False, 2.0, 3))
+    m = scoring()
+    x = z.clone().requires_grad_()
+
+    def step():
+        loss = m.distillation_loss(x, ids, t, 2.0, False, w, reduction)
+        (grad,) = torch.autograd.grad(loss.sum(), x)
+        return loss.detach(), grad
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in (4, 5):
+        with torch.no_grad():
+            x.copy_(case(6, 3001, 12, torch.float16, False, 2.0, seed)[0])
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+def test_teacher_in_sixteen_bits_and_ids_in_32():
+    z, ids, t, w = case(5, 2003, 9, torch.float32, False, 1.0, 12)
+    for dtype in (torch.float16, torch.bfloat16):
+        th = t.to(dtype)
+        loss, grad = scoring().distillation_loss_and_grad(z.cuda(), ids.int().cuda(), th.cuda(), 1.0, False, w.cuda())
+        check(z, ids, th.float(), w, 1.0, False, loss, grad)
+        x = z.cuda().requires_grad_()
+        scoring().distillation_loss(x, ids.int().cuda(), th.cuda(), weights=w.cuda().double()).backward()
+        check(z, ids, th.float(), w, 1.0, False, loss, x.grad)
+
+
 def test_refusals():
     m = scoring()
     z, ids, t, w = (x.cuda() for x in case(4, 100, 5, torch.float32, False, 1.0, 1))

@@ -172,8 +172,32 @@ def test_a_row_that_is_not_finite(fmt):
     assert torch.isnan(m.quantize_fp4(x.cuda(), fmt).dequantize()[2, 100])
 
 
+def test_one_row_without_a_batch_dimension():
+    m = microscale()
+    w = m.quantize_fp4(torch.randn(70, 96, device="cuda"))
+    x = torch.randn(3, 96, device="cuda").half()
+    bias = torch.randn(70, device="cuda").half()
+    y = m.fp4_linear(x, w, bias, out_dtype=torch.float32)
+    assert y.dtype == torch.float32 and torch.equal(m.fp4_linear(x[1], w, bias, out_dtype=torch.float32), y[1])
+    assert torch.equal(m.fp4_linear(x[1:2], w, bias), y[1:2].half()) and torch.equal(y, m.fp4_linear(x, w, bias.float(), out_dtype=torch.float32))
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_a_row_does_not_depend_on_its_batch(fmt):
+    """Tiles, parts along K and kernels change with the number of tokens; what a token gets changes by the order of float32 sums only."""
+    m = microscale()
+    w = m.quantize_fp4(inputs(384, 3000, torch.float32, 2).cuda(), fmt)
+    x = inputs(300, 3000, torch.bfloat16, 1).cuda()
+    packed_rows = m.quantize_fp4(x, fmt)
+    for rows in (1, 16, 17, 33, 65, 128, 129, 300):
+        q = m.quantize_fp4(x[:rows], fmt)
+        assert torch.equal(q.codes, packed_rows.codes[:rows]) and torch.equal(q.block_scales(), packed_rows.block_scales()[:rows])
+        check_product(x[:rows].cpu(), inputs(384, 3000, torch.float32, 2), None, fmt, False, m.fp4_linear(x[:rows], w, out_dtype=torch.float32))
+
+
 def test_no_rows():
     m = microscale()
+    assert m.fp4_linear(torch.ones(3, 32, device="cuda"), m.quantize_fp4(torch.empty(0, 32, device="cuda"))).shape == (3, 0)
     w = m.quantize_fp4(torch.randn(64, 96, device="cuda"))
     assert m.fp4_linear(torch.empty(0, 96, device="cuda"), w).shape == (0, 64)
     assert m.quantize_fp4(torch.empty(0, 96, device="cuda")).dequantize().shape == (0, 96)

@@ -44,7 +44,8 @@ def test_distillation(name):
         return f(*head, saved, loss, total, None) if name == "forward" else f(*head, loss, total, grad, stride, None)
 
     for bad in (dict(logits=None), dict(dtype=3), dict(V=0), dict(plan=None), dict(ids=None), dict(teacher=None), dict(teacher_dtype=-1), dict(K=0), dict(K=513),
-                dict(T=0.0), dict(T=-1.0), dict(T=float("nan")), dict(T=float("inf")), dict(row_loss=None)):
+                dict(T=0.0), dict(T=-1.0), dict(T=float("nan")), dict(T=float("inf")), dict(row_loss=None), dict(ids=C.c_void_p(260)),
+                dict(teacher=C.c_void_p(258))):
         refused(call(**bad))
     for bad in (dict(saved=C.c_void_p(260)),) if name == "forward" else (dict(grad=None), dict(stride=63), dict(total=None), dict(loss=None)):
         refused(call(**bad))
