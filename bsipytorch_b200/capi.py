@@ -75,9 +75,9 @@ SIGNATURES = {
     "bsi_b200_ewah_encode": (_i32, [_vp, _i64, _i64, _f64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp]),
     "bsi_b200_ewah_encode_static": (_i32, [_vp, _i64, _i64, _f64, _vp, _i64, _vp, _vp, _vp, _vp, _vp]),
     "bsi_b200_token_logprobs": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
-    "bsi_b200_distill_forward": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _f32, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp]),
-    "bsi_b200_distill_backward": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _f32, _i32, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp]),
-    "bsi_b200_distill_fused": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _f32, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "bsi_b200_distill_forward": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _f64, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "bsi_b200_distill_backward": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _f64, _i32, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp]),
+    "bsi_b200_distill_fused": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _f64, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),
     "bsi_b200_fp4_scale_bytes": (_i64, [_i64, _i64, _i32]),
     "bsi_b200_fp4_quantize": (_i32, [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _vp, _vp]),
     "bsi_b200_fp4_dequantize": (_i32, [_vp, _i64, _vp, _vp, _i64, _i64, _i32, _vp, _i32, _i64, _vp]),

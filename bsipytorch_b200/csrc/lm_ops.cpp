@@ -154,7 +154,7 @@ struct Teacher {
 };
 
 void check_temperature(double t) {
-    TORCH_CHECK(static_cast<float>(t) > 0.0f && static_cast<float>(t) <= 3.0e38f, "temperature must be positive and finite, got ", t);
+    TORCH_CHECK(t >= 1.0e-30 && t <= 1.0e30, "temperature must be positive (1e-30 to 1e30), got ", t);
 }
 
 // reduction: 0 none, 1 sum, 2 mean
@@ -172,7 +172,7 @@ py::tuple distill_forward(const torch::Tensor& logits, const torch::Tensor& give
     if (reduction != kNone) loss = fresh({}, at::kFloat, dev);
     if (reduction == kMean) sum = fresh({}, at::kFloat, dev);
     check_status(bsi_b200_distill_forward(z.t.data_ptr(), z.code, z.rows, z.V, &z.plan, t.ids.data_ptr<int64_t>(), t.values.data_ptr(), t.code, t.K,
-                                          static_cast<float>(temperature), tail ? 1 : 0, t.weight(), reduction == kMean ? 1 : 0,
+                                          temperature, tail ? 1 : 0, t.weight(), reduction == kMean ? 1 : 0,
                                           row_loss.data_ptr<float>(), save ? saved.data_ptr<float>() : nullptr,
                                           loss.defined() ? loss.data_ptr<float>() : nullptr, sum.defined() ? sum.data_ptr<float>() : nullptr,
                                           current_stream()),
@@ -193,7 +193,7 @@ at::Tensor distill_backward(const torch::Tensor& logits, const torch::Tensor& gi
     const at::Tensor up = upstream.detach().to(at::kFloat).contiguous();
     at::Tensor grad = fresh(with_last(z.lead, z.V), z.t.scalar_type(), z.t.device());
     check_status(bsi_b200_distill_backward(z.t.data_ptr(), z.code, z.rows, z.V, &z.plan, t.ids.data_ptr<int64_t>(), t.values.data_ptr(), t.code, t.K,
-                                           static_cast<float>(temperature), tail ? 1 : 0, t.weight(), saved.data_ptr<float>(),
+                                           temperature, tail ? 1 : 0, t.weight(), saved.data_ptr<float>(),
                                            up.data_ptr<float>(), up.numel() == 1 ? 0 : 1, sum.has_value() ? sum->data_ptr<float>() : nullptr,
                                            grad.data_ptr(), z.V, current_stream()),
                  "bsi_b200_distill_backward");
@@ -210,7 +210,7 @@ py::tuple distill_fused(const torch::Tensor& logits, const torch::Tensor& given_
     at::Tensor row_loss = fresh(z.lead, at::kFloat, dev), loss = fresh({}, at::kFloat, dev), sum = fresh({}, at::kFloat, dev);
     at::Tensor grad = fresh(with_last(z.lead, z.V), z.t.scalar_type(), dev);
     check_status(bsi_b200_distill_fused(z.t.data_ptr(), z.code, z.rows, z.V, &z.plan, t.ids.data_ptr<int64_t>(), t.values.data_ptr(), t.code, t.K,
-                                        static_cast<float>(temperature), tail ? 1 : 0, t.weight(), reduction == kMean ? 1 : 0,
+                                        temperature, tail ? 1 : 0, t.weight(), reduction == kMean ? 1 : 0,
                                         row_loss.data_ptr<float>(), loss.data_ptr<float>(), sum.data_ptr<float>(), grad.data_ptr(), z.V,
                                         current_stream()),
                  "bsi_b200_distill_fused");

@@ -3,6 +3,7 @@
 // Both need the softmax statistics of every row, so both are one pass over the logits with a running maximum and sum per thread
 // (vocab.cuh), joined in a block and then in a cluster. What bounds them is the logits' bytes.
 #include <algorithm>
+#include <cmath>
 
 #include "vocab.cuh"
 
@@ -24,6 +25,7 @@ int take_vocab_status(int* v) {
 namespace {
 
 namespace cg = cooperative_groups;
+__device__ __forceinline__ vocab::Factor natural() { return vocab::Factor{1.44269502162933349609375f, 1.92596299e-8f}; }      // log2(e)
 using vocab::kBatch;
 using vocab::kChunk;
 using vocab::kThreads;
@@ -199,7 +201,7 @@ struct ScoreThread {
 
     template <int B>
     __device__ __forceinline__ float take(const uint4 (&u)[B], int v) {
-        const float top = run.take(u, vocab::kLog2e);
+        const float top = run.take(u, natural());
         typename Piece<T>::Count count;
 #pragma unroll
         for (int b = 0; b < B; ++b) count.add(u[b], v + b * kThreads < token_piece ? at : behind);
@@ -329,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) score_kernel(const ScoreArgs
 
     // the block's statistics
     __syncwarp();
-    Stats all = vocab::warp_merge(me.run.stats(vocab::kLog2e), vocab::kLog2e);
+    Stats all = vocab::warp_merge(me.run.stats(natural()), natural());
     const int ahead = __reduce_add_sync(0xFFFFFFFFu, me.ahead);
     if (lane == 0) {
         sh.warp[warp] = all;
@@ -338,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) score_kernel(const ScoreArgs
     __syncthreads();
     if (warp == 0) {
         all = lane < kWarps ? sh.warp[lane] : Stats{-CUDART_INF_F, 0.0f, 0.0f};
-        all = vocab::warp_merge(all, vocab::kLog2e);
+        all = vocab::warp_merge(all, natural());
         const int n = __reduce_add_sync(0xFFFFFFFFu, lane < kWarps ? sh.warp_ahead[lane] : 0);
         if (lane == 0) {
             sh.mine = all;
@@ -394,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) score_kernel(const ScoreArgs
             // the others' statistics, a lane each, and lists, all at once
             if (warp == 0) {
                 const ScoreShared* other = cluster.map_shared_rank(&sh, min(lane, parts - 1));
-                const Stats total = vocab::warp_merge(lane < parts ? other->mine : Stats{-CUDART_INF_F, 0.0f, 0.0f}, vocab::kLog2e);
+                const Stats total = vocab::warp_merge(lane < parts ? other->mine : Stats{-CUDART_INF_F, 0.0f, 0.0f}, natural());
                 const int before = __reduce_add_sync(0xFFFFFFFFu, lane < parts ? other->ahead : 0);
                 if (lane < parts) sh.lengths[lane] = other->listed;
                 __syncwarp();
@@ -555,7 +557,8 @@ struct DistillArgs {
     const void* teacher;         // [rows, K]
     int teacher_dtype;
     int K;
-    float temperature;
+    vocab::Factor c;             // log2(e) / T
+    double temperature;
     int tail;
     const float* weights;        // [rows] or null
     float* row_loss;             // [rows], weight and T^2 included
@@ -580,7 +583,7 @@ struct DistillShared {
     float part[kWarps];
     vocab::Feed feed;
     Stats rest, listed;          // of this CTA's part of the row, read by the other CTAs
-    float total_p;
+    float total_p, rest_p;             // the entries' probabilities summed, and what they leave of 1
     long long raw_id[kMaxListed];      // as they lie in memory
     float raw_t[kMaxListed];
     uint32_t raw_z[kMaxListed];
@@ -623,10 +626,10 @@ __device__ __forceinline__ void ask_logits(DistillShared& sh, const DistillArgs&
         if (there) copy_async(&sh.raw_z[k], reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(row + id) & ~uintptr_t(3)), false);
     }
 }
+// A handful of values a row, of whose differences the gradient is made: in double.
 template <typename T>
 __device__ void finish_entries(DistillShared& sh, const DistillArgs& a, int64_t r, const T* row) {
     const int lane = threadIdx.x & 31;
-    const float inv_t = 1.0f / a.temperature;
     copies_done();
     float top = -CUDART_INF_F;
     for (int k = lane; k < a.K; k += 32) {
@@ -642,34 +645,36 @@ __device__ void finish_entries(DistillShared& sh, const DistillArgs& a, int64_t 
                 z = Piece<T>::one(*reinterpret_cast<const T*>(&half));
             }
         }
-        if (!a.tail) t *= inv_t;
         sh.entry[k].logp = t;
         sh.entry[k].z = z;
         top = vocab::max_nan(top, t);
     }
-    float norm = 0.0f;
-    if (!a.tail) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = vocab::max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        float s = 0.0f;
-        if (top != -CUDART_INF_F) {
-            for (int k = lane; k < a.K; k += 32) s += expf(sh.entry[k].logp - top);
-        }
+    for (int o = 16; o > 0; o >>= 1) top = vocab::max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    const double scale = a.tail ? 1.0 : 1.0 / a.temperature;
+    // log p = (t - top) / T - log sum exp((t - top) / T), or t as it is
+    const double from = a.tail || top == -CUDART_INF_F ? 0.0 : static_cast<double>(top);
+    double norm = 0.0;
+    if (!a.tail && top != -CUDART_INF_F) {
+        double s = 0.0;
+        for (int k = lane; k < a.K; k += 32) s += exp((sh.entry[k].logp - from) * scale);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-        norm = top == -CUDART_INF_F ? 0.0f : top + logf(s);
+        norm = log(s);
     }
-    float sum = 0.0f;
+    double sum = 0.0;
     for (int k = lane; k < a.K; k += 32) {
-        const float lp = sh.entry[k].logp - norm;
-        const float p = expf(lp);
-        sh.entry[k].logp = lp;
-        sh.entry[k].p = p;
+        const double lp = (sh.entry[k].logp - from) * scale - norm, p = exp(lp);
+        sh.entry[k].logp = static_cast<float>(lp);
+        sh.entry[k].p = static_cast<float>(p);
         sum += p;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    if (lane == 0) sh.total_p = sum;
+    if (lane == 0) {
+        sh.total_p = static_cast<float>(sum);
+        sh.rest_p = static_cast<float>(1.0 - sum);
+    }
 }
 
 // One value per thread summed over the block, the same on every call with the same values.
@@ -707,11 +712,13 @@ struct Gradient {
     static constexpr int kVec = Piece<T>::kVec;
     T* out;
     uint4* out_grid;
-    float c, m, rest, top, scale;
+    vocab::Factor c;
+    double inv_t;
+    float m, rest, top, scale;
     bool vector, on;
 
     __device__ __forceinline__ Gradient(const DistillArgs& a, uint32_t r, const Span<T>& span, const float4& saved, float s)
-        : out(static_cast<T*>(a.grad) + r * a.grad_stride), c(vocab::kLog2e / a.temperature), m(saved.x), rest(s * saved.z * saved.y), top(s * saved.y),
+        : out(static_cast<T*>(a.grad) + r * a.grad_stride), c(a.c), inv_t(1.0 / a.temperature), m(saved.x), rest(s * saved.z * saved.y), top(s * saved.y),
           scale(s), vector((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(T) == static_cast<unsigned>(span.shift)), on(saved.w != 0.0f && s != 0.0f) {
         out_grid = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(out) & ~uintptr_t(15));
     }
@@ -719,11 +726,12 @@ struct Gradient {
         float z[kVec];
         if (on) {
             Piece<T>::unpack(u, z);
-            const vocab::Two less(-m, -m), cc(c, c), rr(rest, rest);
+            const vocab::Two less(-m, -m), cc(c.hi, c.hi), ll(c.lo, c.lo), rr(rest, rest);
 #pragma unroll
             for (int e = 0; e < kVec; e += 2) {
                 float d0, d1;
-                vocab::mul2(vocab::add2(vocab::Two(z[e], z[e + 1]), less), cc).split(d0, d1);
+                const vocab::Two x = vocab::add2(vocab::Two(z[e], z[e + 1]), less);
+                vocab::fma2(x, ll, vocab::mul2(x, cc)).split(d0, d1);
                 vocab::mul2(vocab::Two(vocab::exp2_fast(d0), vocab::exp2_fast(d1)), rr).split(z[e], z[e + 1]);
             }
         } else {
@@ -767,7 +775,8 @@ struct Gradient {
             if (id < lo || id >= hi) continue;
             float p;
             if (!first_of_id(sh, K, k, &p)) continue;
-            out[id] = Piece<T>::narrow(top * vocab::exp2_fast((sh.entry[k].z - m) * c) - scale * p);
+            const double q = exp((static_cast<double>(sh.entry[k].z) - m) * inv_t);
+            out[id] = Piece<T>::narrow(static_cast<float>(top * q - static_cast<double>(scale) * p));
         }
     }
 };
@@ -777,7 +786,7 @@ __device__ __forceinline__ float grad_scale(const DistillArgs& a, int64_t r) {
     const float up = a.upstream != nullptr ? a.upstream[r * a.upstream_stride] : 1.0f;
     const float d = a.denominator != nullptr ? *a.denominator : 1.0f;
     if (w == 0.0f || d == 0.0f) return 0.0f;
-    return up * a.temperature * (w / d);
+    return up * static_cast<float>(a.temperature) * (w / d);
 }
 
 // The forward pass; GRAD: the gradient too, while L2 still holds the row. Dynamic shared memory: with the tail on, one bit per logit of
@@ -827,7 +836,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const Distill
 
     // The last warp has the entries
     if (warp == kWarps - 1) ask_logits<T>(sh, a, row);
-    const float c = vocab::kLog2e / a.temperature;
+    const vocab::Factor c = a.c;
     const int bit0 = span.element(span.first);         // the part's bit 0; kVec bits for each piece
     const int lo = span.begin(), hi = span.end();
     if (a.tail) {
@@ -943,10 +952,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const Distill
         outside = block_sum(distinct, sh.part) < static_cast<float>(a.V);
     }
     const float log_s = logf(all.s);
-    const float inv_t = 1.0f / a.temperature;
-    const float p_rest = a.tail ? fmaxf(1.0f - sh.total_p, 0.0f) : 0.0f;
+    const double inv_t = 1.0 / a.temperature;
+    const float p_rest = a.tail ? fmaxf(sh.rest_p, 0.0f) : 0.0f;
     // log of the rest's share, from its own maximum and sum; nothing there: the share is 0
-    const float log_rest = rest.s != 0.0f ? (rest.m - all.m) * inv_t + logf(rest.s) - log_s : -CUDART_INF_F;
+    const float log_rest = rest.s != 0.0f ? static_cast<float>((static_cast<double>(rest.m) - all.m) * inv_t) + logf(rest.s / all.s) : -CUDART_INF_F;
     float factor = 1.0f;
     if (a.tail && rest.s != 0.0f) factor = 1.0f - p_rest * expf(-log_rest);
     // a row without any entry has no loss and no gradient
@@ -956,13 +965,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const Distill
         float loss = 0.0f;
         for (int k = tid; k < a.K; k += kThreads) {
             const Entry e = sh.entry[k];
-            if (e.id >= 0 && e.p != 0.0f) loss += e.p * (e.logp - ((e.z - all.m) * inv_t - log_s));
+            if (e.id >= 0 && e.p != 0.0f) loss += e.p * static_cast<float>(e.logp - ((static_cast<double>(e.z) - all.m) * inv_t - log_s));
         }
         loss = block_sum(loss, sh.part);
         if (tid == 0) {
             if (p_rest != 0.0f && outside) loss += p_rest * (logf(p_rest) - log_rest);
             const float w = a.weights != nullptr ? a.weights[r] : 1.0f;
-            a.row_loss[r] = loss * (a.temperature * a.temperature) * w;
+            a.row_loss[r] = loss * static_cast<float>(a.temperature * a.temperature) * w;
             if (a.saved != nullptr) a.saved[r] = saved;
         }
     }
@@ -1071,8 +1080,16 @@ int launch_distill_backward(const DistillArgs& a, int64_t rows, cudaStream_t str
     return check_launch("distill_backward launch");
 }
 
+vocab::Factor factor_of(double temperature) {
+    // the upper part rounded down and never the whole: -inf times the lower one is -inf, not NaN
+    const double c = 1.4426950408889634074 / temperature;
+    float hi = static_cast<float>(c);
+    if (static_cast<double>(hi) >= c) hi = std::nextafter(hi, 0.0f);
+    return vocab::Factor{hi, static_cast<float>(c - hi)};
+}
+
 int check_distill(const char* what, const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan, const int64_t* ids,
-                  const void* teacher, int teacher_dtype, int K, float temperature) {
+                  const void* teacher, int teacher_dtype, int K, double temperature) {
     const int rc = check_rows(what, logits, dtype, rows, V, plan);
     if (rc != BSI_OK) return rc;
     if (K < 1 || K > kMaxListed) {
@@ -1091,8 +1108,8 @@ int check_distill(const char* what, const void* logits, int dtype, int64_t rows,
         set_error("%s: misaligned ids or teacher", what);
         return BSI_ERR_INVALID;
     }
-    if (!(temperature > 0.0f) || !(temperature <= 3.0e38f)) {
-        set_error("%s: temperature must be positive and finite", what);
+    if (!(temperature >= 1.0e-30) || !(temperature <= 1.0e30)) {
+        set_error("%s: temperature must lie in [1e-30, 1e30]", what);
         return BSI_ERR_INVALID;
     }
     return BSI_OK;
@@ -1128,7 +1145,7 @@ extern "C" int bsi_b200_token_logprobs(const void* logits, int dtype, int64_t ro
 }
 
 extern "C" int bsi_b200_distill_forward(const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan,
-                                        const int64_t* ids, const void* teacher, int teacher_dtype, int K, float temperature, int tail,
+                                        const int64_t* ids, const void* teacher, int teacher_dtype, int K, double temperature, int tail,
                                         const float* weights, int mean, float* row_loss, float* saved, float* loss, float* weight_sum,
                                         bsi_stream_t stream) {
     using namespace bsi;
@@ -1139,7 +1156,7 @@ extern "C" int bsi_b200_distill_forward(const void* logits, int dtype, int64_t r
     rc = require_sm100();
     if (rc != BSI_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, temperature, tail != 0, weights, row_loss,
+    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, factor_of(temperature), temperature, tail != 0, weights, row_loss,
                   reinterpret_cast<float4*>(saved), nullptr, 0, nullptr, nullptr, 0};
     if (rows > 0) {
         rc = dtype == BSI_DTYPE_F32 ? launch_distill<float, false>(a, rows, s)
@@ -1152,7 +1169,7 @@ extern "C" int bsi_b200_distill_forward(const void* logits, int dtype, int64_t r
 }
 
 extern "C" int bsi_b200_distill_backward(const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan,
-                                         const int64_t* ids, const void* teacher, int teacher_dtype, int K, float temperature, int tail,
+                                         const int64_t* ids, const void* teacher, int teacher_dtype, int K, double temperature, int tail,
                                          const float* weights, const float* saved, const float* upstream, int64_t upstream_stride,
                                          const float* denominator, void* grad, int64_t grad_stride, bsi_stream_t stream) {
     using namespace bsi;
@@ -1165,14 +1182,14 @@ extern "C" int bsi_b200_distill_backward(const void* logits, int dtype, int64_t 
     rc = require_sm100();
     if (rc != BSI_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, temperature, tail != 0, weights, nullptr,
+    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, factor_of(temperature), temperature, tail != 0, weights, nullptr,
                   const_cast<float4*>(reinterpret_cast<const float4*>(saved)), upstream, upstream_stride, denominator, grad, grad_stride};
     return dtype == BSI_DTYPE_F32 ? launch_distill_backward<float>(a, rows, s)
            : dtype == BSI_DTYPE_F16 ? launch_distill_backward<__half>(a, rows, s) : launch_distill_backward<__nv_bfloat16>(a, rows, s);
 }
 
 extern "C" int bsi_b200_distill_fused(const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan,
-                                      const int64_t* ids, const void* teacher, int teacher_dtype, int K, float temperature, int tail,
+                                      const int64_t* ids, const void* teacher, int teacher_dtype, int K, double temperature, int tail,
                                       const float* weights, int mean, float* row_loss, float* loss, float* weight_sum,
                                       void* grad, int64_t grad_stride, bsi_stream_t stream) {
     using namespace bsi;
@@ -1189,7 +1206,7 @@ extern "C" int bsi_b200_distill_fused(const void* logits, int dtype, int64_t row
         rc = check_launch("distill weights launch");
         if (rc != BSI_OK) return rc;
     }
-    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, temperature, tail != 0, weights, row_loss,
+    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, factor_of(temperature), temperature, tail != 0, weights, row_loss,
                   nullptr, nullptr, 0, mean ? weight_sum : nullptr, grad, grad_stride};
     if (rows > 0) {
         rc = dtype == BSI_DTYPE_F32 ? launch_distill<float, true>(a, rows, s)

@@ -25,7 +25,6 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kBatch = 4;               // 16-byte pieces that a thread has under way
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // Rows of a 2-D or 3-D tensor: row r lies at (r / per) * block + (r % per) * row elements.
@@ -298,12 +297,18 @@ struct Stats {
     float m, s, w;
 };
 
-// Two sets of statistics as one. c: scale * log2(e).
-__device__ __forceinline__ Stats merge(const Stats& a, const Stats& b, float c) {
+// scale * log2(e) in two parts, both above 0: a rounded factor alone would be off by 2^-25 of itself, which exponents of 30 turn into 1e-6 of a weight.
+struct Factor {
+    float hi, lo;
+    __device__ __forceinline__ float times(float x) const { return fmaf(x, lo, x * hi); }
+};
+
+// Two sets of statistics as one.
+__device__ __forceinline__ Stats merge(const Stats& a, const Stats& b, const Factor& c) {
     Stats r;
     r.m = max_nan(a.m, b.m);
     if (r.m == -CUDART_INF_F) return Stats{-CUDART_INF_F, 0.0f, 0.0f};
-    const float da = a.m == -CUDART_INF_F ? 0.0f : (a.m - r.m) * c, db = b.m == -CUDART_INF_F ? 0.0f : (b.m - r.m) * c;
+    const float da = a.m == -CUDART_INF_F ? 0.0f : c.times(a.m - r.m), db = b.m == -CUDART_INF_F ? 0.0f : c.times(b.m - r.m);
     const float fa = exp2_fast(da), fb = exp2_fast(db);
     // a side without any mass adds nothing, however far below it lies
     r.s = (a.s != 0.0f ? a.s * fa : 0.0f) + (b.s != 0.0f ? b.s * fb : 0.0f);
@@ -312,12 +317,12 @@ __device__ __forceinline__ Stats merge(const Stats& a, const Stats& b, float c) 
 }
 
 // The warp's statistics as one: their maximum first, then sums against it.
-__device__ __forceinline__ Stats warp_merge(const Stats& v, float c) {
+__device__ __forceinline__ Stats warp_merge(const Stats& v, const Factor& c) {
     float m = v.m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
     if (m == -CUDART_INF_F) return Stats{m, 0.0f, 0.0f};
-    const float d = v.s != 0.0f ? (v.m - m) * c : 0.0f;
+    const float d = v.s != 0.0f ? c.times(v.m - m) : 0.0f;
     const float f = exp2_fast(d);
     // a side without any mass adds nothing, however far below it lies
     float s = v.s != 0.0f && f != 0.0f ? v.s * f : 0.0f, w = v.s != 0.0f && f != 0.0f ? f * fmaf(d, v.s, v.w) : 0.0f;
@@ -470,7 +475,8 @@ struct Running {
     __device__ __forceinline__ Running() : m(-INFINITY), base(NAN), s(0.0f), w(0.0f), far(false) {}      // no value passes a NaN: the first batch sets base
 
     // A new reference at a new maximum.
-    __device__ __forceinline__ void raise(float top, float c) {
+    __device__ __forceinline__ void raise(float top, const Factor& factor) {
+        const float c = factor.hi;
         const float old_m = m, old_base = base;
         const bool old_far = far;
         base = rintf(top * c);
@@ -488,15 +494,16 @@ struct Running {
 
     // Returns the largest of the values.
     template <int B>
-    __device__ __forceinline__ float take(const uint4 (&u)[B], float c) {
+    __device__ __forceinline__ float take(const uint4 (&u)[B], const Factor& factor) {
         constexpr int kVec = Piece<T>::kVec;
+        const float c = factor.hi;
         const float top = Piece<T>::top(u);
-        if (far ? !(top <= m) : !(fmaf(top, c, -32.0f) <= base)) raise(top, c);      // far higher, or a NaN
+        if (far ? !(top <= m) : !(fmaf(top, c, -32.0f) <= base)) raise(top, factor);      // far higher, or a NaN
         m = max_nan(m, top);
         if (m == -CUDART_INF_F) return top;       // nothing but -inf so far
         float s0 = 0.0f, s1 = 0.0f, w0 = 0.0f, w1 = 0.0f;
         if (!far) {
-            const Two cc(c, c), bb(-base, -base);
+            const Two cc(c, c), ll(factor.lo, factor.lo), bb(-base, -base);
             Two ss(0.0f, 0.0f), ww(0.0f, 0.0f);
 #pragma unroll
             for (int b = 0; b < B; ++b) {
@@ -504,7 +511,9 @@ struct Running {
                 Piece<T>::unpack(W ? Piece<T>::finite_floor(u[b]) : u[b], z);
 #pragma unroll
                 for (int e = 0; e < kVec; e += 2) {
-                    const Two d = fma2(Two(z[e], z[e + 1]), cc, bb);
+                    const Two x01(z[e], z[e + 1]);
+                    Two d = fma2(x01, cc, bb);
+                    if (!W) d = fma2(x01, ll, d);      // the entropy's statistics have the factor log2(e), whose float32 is good to 2^-26
                     float d0, d1;
                     d.split(d0, d1);
                     const Two x(exp2_fast(d0), exp2_fast(d1));
@@ -535,10 +544,10 @@ struct Running {
     }
 
     // Against m, as merge() takes them.
-    __device__ __forceinline__ Stats stats(float c) const {
+    __device__ __forceinline__ Stats stats(const Factor& c) const {
         if (m == -CUDART_INF_F) return Stats{m, 0.0f, 0.0f};
         if (far) return Stats{m, s, w};
-        const float d = -fmaf(m, c, -base);       // base - m * c, down to -32
+        const float d = -fmaf(m, W ? 0.0f : c.lo, fmaf(m, c.hi, -base));       // base - m * c, down to -32
         const float f = exp2_fast(d);
         return Stats{m, s * f, W ? f * fmaf(d, s, w) : 0.0f};
     }

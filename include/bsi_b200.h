@@ -467,20 +467,20 @@ int bsi_b200_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t
  * mean != 0: divided by the weights' sum (0 where that is 0), which weight_sum receives. row_loss [rows]: the rows' weighted losses.
  * saved [rows, 4] float32, 16-byte aligned: what the backward pass takes. loss, weight_sum and saved may be NULL. */
 int bsi_b200_distill_forward(const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan,
-                             const int64_t* ids, const void* teacher, int teacher_dtype, int K, float temperature, int tail,
+                             const int64_t* ids, const void* teacher, int teacher_dtype, int K, double temperature, int tail,
                              const float* weights, int mean, float* row_loss, float* saved, float* loss, float* weight_sum,
                              bsi_stream_t stream);
 /* grad [rows, V] in the logits' type, rows grad_stride >= V apart, not overlapping the logits:
  * upstream[r * upstream_stride] * weights[r] / *denominator * dloss_r/dz. upstream and denominator may be NULL (1); a denominator of 0
  * gives a gradient of 0. */
 int bsi_b200_distill_backward(const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan,
-                              const int64_t* ids, const void* teacher, int teacher_dtype, int K, float temperature, int tail,
+                              const int64_t* ids, const void* teacher, int teacher_dtype, int K, double temperature, int tail,
                               const float* weights, const float* saved, const float* upstream, int64_t upstream_stride,
                               const float* denominator, void* grad, int64_t grad_stride, bsi_stream_t stream);
 /* Both at once, the logits read from memory once: a row's second reading comes out of L2. Same loss, and the gradient of `loss`. loss
  * and weight_sum are needed. */
 int bsi_b200_distill_fused(const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan,
-                           const int64_t* ids, const void* teacher, int teacher_dtype, int K, float temperature, int tail,
+                           const int64_t* ids, const void* teacher, int teacher_dtype, int K, double temperature, int tail,
                            const float* weights, int mean, float* row_loss, float* loss, float* weight_sum,
                            void* grad, int64_t grad_stride, bsi_stream_t stream);
 
