@@ -50,7 +50,7 @@ static_assert(vocab::kMaxCluster * kMaxTop <= kCandidates, "CTA 0 gathers the ot
 //
 // The top k ride on the same pass. Every warp knows the j-th largest of its lanes' running maxima, j = ceil(k / 8); with B the t-th
 // largest of these over the 8 warps, t = ceil(k / j), at least k entries are >= B, so the k largest all are, and few others. It is
-// worked out behind chunks 1, 2, 4, 8, ... without any barrier, as a bound of an earlier time is one too; a thread only notes which of
+// worked out behind chunks 1, 2, 3, 4, 8, 16, ... without any barrier, as a bound of an earlier time is one too; a thread only notes which of
 // its batches reached the bound of their time, a bit each. At the row's end the last bound is a tight one, and the few batches noted
 // are read again, out of L2, for the entries that reach it, which are put in order by counting for each one how many come before it.
 // (633 x 128011 float32, k = 64: keeping the entries themselves as the row goes by took 138 us, reading again all that a thread whose
@@ -288,7 +288,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) score_kernel(const ScoreArgs
     // bit: one batch, or as many as 64 bits have to share (rows of more than a megabyte a part)
     const int share = (pieces + 64 * kChunk - 1) / (64 * kChunk);
     unsigned long long noted = 0;
-    float first_largest = -CUDART_INF_F;
+    // the batches with the four highest maxima of those noted: place << 16 | bit, descending; lost: the highest place that did not fit
+    uint32_t best_batch[4] = {0u, 0u, 0u, 0u}, lost = 0;
     for (int i = 0, n = 0; i < pieces; i += kChunk, ++n) {
         const uint4* chunk = ring.arrive(place);
         const int v = span.whole_first() + i + tid;
@@ -309,9 +310,19 @@ __global__ void __launch_bounds__(kThreads, kPerSm) score_kernel(const ScoreArgs
         ring.release(place);
         ring.advance(place);
         if (top) {
-            if (n == 0) first_largest = largest;
-            else if (!(largest < me.bound)) noted |= 1ull << (n / share);
-            if ((n & (n + 1)) == 0) {
+            if (n == 0 || !(largest < me.bound)) {
+                const int bit = n / share;
+                noted |= 1ull << bit;
+                uint32_t in = Piece<T>::place(largest) << 16 | static_cast<uint32_t>(bit);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t low = min(best_batch[q], in);
+                    best_batch[q] = max(best_batch[q], in);
+                    in = low;
+                }
+                lost = max(lost, in >> 16);
+            }
+            if ((n & (n + 1)) == 0 || n == 2) {
                 const uint32_t all = publish();
                 if (lane == 0) atomicMax(&sh.agreed_bound, all);
             }
@@ -349,18 +360,27 @@ __global__ void __launch_bounds__(kThreads, kPerSm) score_kernel(const ScoreArgs
     }
 
     if (top) {
-        me.set_bound(sh.agreed(voters, t));
-        if (!(first_largest < me.bound)) noted |= 1ull;
-        while (noted != 0ull) {
-            const int bit = __ffsll(static_cast<long long>(noted)) - 1;
-            noted &= noted - 1ull;
-            for (int n = bit * share; n < (bit + 1) * share && n * kChunk + tid < pieces; ++n) {
-                const int v = span.whole_first() + n * kChunk + tid;
-                uint4 u[kBatch];
+        const uint32_t last_bound = max(sh.agreed(voters, t), Piece<T>::kFloor);
+        me.set_bound(last_bound);
+        auto look_again = [&](int n) {
+            const int v = span.whole_first() + n * kChunk + tid;
+            if (v >= span.whole_last()) return;
+            uint4 u[kBatch];
 #pragma unroll
-                for (int b = 0; b < kBatch; ++b)
-                    u[b] = v + b * kThreads < span.whole_last() ? span.grid[v + b * kThreads] : make_uint4(Piece<T>::kNone, Piece<T>::kNone, Piece<T>::kNone, Piece<T>::kNone);
-                me.keep(sh, span, u, v, Piece<T>::top(u), row + span.element(v));
+            for (int b = 0; b < kBatch; ++b)
+                u[b] = v + b * kThreads < span.whole_last() ? span.grid[v + b * kThreads] : make_uint4(Piece<T>::kNone, Piece<T>::kNone, Piece<T>::kNone, Piece<T>::kNone);
+            me.keep(sh, span, u, v, Piece<T>::top(u), row + span.element(v));
+        };
+        if (share == 1 && lost < last_bound) {
+            // a thread has seldom more than one or two of them: each look takes memory's whole latency
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (best_batch[q] >> 16 >= last_bound) look_again(static_cast<int>(best_batch[q] & 63u));
+        } else if (Piece<T>::place(me.run.m) >= last_bound) {
+            while (noted != 0ull) {
+                const int bit = __ffsll(static_cast<long long>(noted)) - 1;
+                noted &= noted - 1ull;
+                for (int n = bit * share; n < (bit + 1) * share; ++n) look_again(n);
             }
         }
         if ((tid == 0 && span.has_left()) || (tid == 32 && span.has_right())) {
@@ -383,6 +403,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) score_kernel(const ScoreArgs
         for (int i = tid; i < n; i += kThreads) {
             const unsigned long long key = sh.cand[i];
             int place = 0;
+#pragma unroll 8
             for (int q = 0; q < n; ++q) place += sh.cand[q] > key;
             if (place < k) sh.best[place] = key;
         }
@@ -446,27 +467,21 @@ __global__ void __launch_bounds__(kThreads, kPerSm) score_kernel(const ScoreArgs
     }
 }
 
-// CTAs per row and rows under way: as many CTAs as the GPU holds walk over the rows. An SM takes its share of them at its share of the
-// memory's rate, 42 bytes per ns, unless a CTA's own pace holds it up: 20 bytes per ns, and the end of a row, 4 us, or 8 where a cluster
-// has to join its parts. The number of parts for which that is shortest. (633 x 128011 float32: one part 70 us, two 117.)
+// CTAs per row and rows under way: as many CTAs as the GPU holds walk over the rows. A row by itself is read at 20 bytes per ns and CTA,
+// so few rows are shared by clusters (one row of 128011 float32: 31.5 us alone, 8.8 by eight CTAs); but a cluster joins its parts at the
+// row's end, and where rows follow one another that costs more than it gives (512 rows: 52 us alone, 57 by two, 124 by eight). Shared as
+// long as every part has 8 KB and the parts are no more than two to an SM, or four with 96 KB each. Eight lists of many alternatives
+// are joined more slowly than they are found (64 of one row: 14.5 us by four, 17.9 by eight; 20: 16.7 and 14.8).
 struct Walk {
     int parts;
     int64_t clusters;
 };
-Walk walk_over(int64_t rows, int64_t V, int esz, int least_parts, int per_sm) {
-    const int64_t sms = sm_count();
-    Walk best{0, 0};
-    double least = 0.0;
-    for (int parts = least_parts; parts <= vocab::kMaxCluster; parts *= 2) {
-        const double bytes = static_cast<double>(V) * esz / parts, end = parts > 1 ? 8.0 : 4.0;
-        const int64_t mine = (rows * parts + sms - 1) / sms, rounds = (mine + per_sm - 1) / per_sm;       // of one SM
-        const double cost = std::max(static_cast<double>(mine) * bytes / 42000.0 + end, static_cast<double>(rounds) * (bytes / 20000.0 + end));
-        if (best.parts == 0 || cost < least) {
-            least = cost;
-            best = Walk{parts, std::min(rows, std::max<int64_t>(1, sms * per_sm / parts))};
-        }
-    }
-    return best;
+Walk walk_over(int64_t rows, int64_t V, int esz, int least_parts, int most_parts, int per_sm) {
+    const int64_t sms = sm_count(), bytes = V * esz;
+    int parts = least_parts;
+    while (parts * 2 <= most_parts && bytes >= 8192 * parts * 2 &&
+           (rows * parts * 2 <= 2 * sms || (rows * parts * 2 <= 4 * sms && bytes >= 98304 * parts * 2))) parts *= 2;
+    return Walk{parts, std::min(rows, std::max<int64_t>(1, sms * per_sm / parts))};
 }
 
 template <typename Kernel, typename... Args>
@@ -507,7 +522,7 @@ template <typename T>
 int launch_score(const ScoreArgs& a, int64_t rows, cudaStream_t stream) {
     static bool set[64] = {false};
     if (int rc = allow_shared(score_kernel<T>, kRingBytes, set)) return rc;
-    return launch_rows(score_kernel<T>, walk_over(rows, a.V, sizeof(T), 1, kPerSm), kRingBytes, stream, "token_logprobs", a);
+    return launch_rows(score_kernel<T>, walk_over(rows, a.V, sizeof(T), 1, a.top > 32 ? 4 : vocab::kMaxCluster, kPerSm), kRingBytes, stream, "token_logprobs", a);
 }
 
 constexpr int64_t kMaxRows = 0x7FFFFFFFll / vocab::kMaxCluster;
@@ -558,7 +573,7 @@ struct DistillArgs {
     int teacher_dtype;
     int K;
     vocab::Factor c;             // log2(e) / T
-    double temperature;
+    double temperature, inv_t;
     int tail;
     const float* weights;        // [rows] or null
     float* row_loss;             // [rows], weight and T^2 included
@@ -578,12 +593,19 @@ struct Entry {
     float z;
 };
 
+// A row's softmax: maximum, 1 / sum, the factor of q outside the list, log of the sum, log of what is not listed's share.
+struct Joined {
+    float m, inv_s, factor, log_s, log_share;
+};
+
 struct DistillShared {
     Stats warp[kWarps], warp_listed[kWarps];
     float part[kWarps];
     vocab::Feed feed;
     Stats rest, listed;          // of this CTA's part of the row, read by the other CTAs
-    float total_p, rest_p;             // the entries' probabilities summed, and what they leave of 1
+    Joined joined;
+    double rest_p;                     // what the entries' probabilities leave of 1
+    float total_p;                     // their sum
     long long raw_id[kMaxListed];      // as they lie in memory
     float raw_t[kMaxListed];
     uint32_t raw_z[kMaxListed];
@@ -651,7 +673,7 @@ __device__ void finish_entries(DistillShared& sh, const DistillArgs& a, int64_t 
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = vocab::max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    const double scale = a.tail ? 1.0 : 1.0 / a.temperature;
+    const double scale = a.tail ? 1.0 : a.inv_t;
     // log p = (t - top) / T - log sum exp((t - top) / T), or t as it is
     const double from = a.tail || top == -CUDART_INF_F ? 0.0 : static_cast<double>(top);
     double norm = 0.0;
@@ -673,7 +695,7 @@ __device__ void finish_entries(DistillShared& sh, const DistillArgs& a, int64_t 
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     if (lane == 0) {
         sh.total_p = static_cast<float>(sum);
-        sh.rest_p = static_cast<float>(1.0 - sum);
+        sh.rest_p = 1.0 - sum;
     }
 }
 
@@ -718,7 +740,7 @@ struct Gradient {
     bool vector, on;
 
     __device__ __forceinline__ Gradient(const DistillArgs& a, uint32_t r, const Span<T>& span, const float4& saved, float s)
-        : out(static_cast<T*>(a.grad) + r * a.grad_stride), c(a.c), inv_t(1.0 / a.temperature), m(saved.x), rest(s * saved.z * saved.y), top(s * saved.y),
+        : out(static_cast<T*>(a.grad) + r * a.grad_stride), c(a.c), inv_t(a.inv_t), m(saved.x), rest(s * saved.z * saved.y), top(s * saved.y),
           scale(s), vector((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(T) == static_cast<unsigned>(span.shift)), on(saved.w != 0.0f && s != 0.0f) {
         out_grid = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(out) & ~uintptr_t(15));
     }
@@ -941,8 +963,21 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const Distill
         }
         __syncthreads();
     }
-    const Stats rest = sh.rest;
-    const Stats all = a.tail ? vocab::merge(rest, sh.listed, c) : rest;
+    if (a.tail) {
+        // What is listed and what is not, joined in double by one thread: the gradient of what is not listed goes with 1 - rest / q_rest,
+        // which is small where the teacher's rest and the student's are alike.
+        if (tid == 0) {
+            const Stats rest = sh.rest, in = sh.listed;
+            const float m = vocab::max_nan(rest.m, in.m);
+            const double r_s = rest.s != 0.0f ? rest.s * exp((static_cast<double>(rest.m) - m) * a.inv_t) : 0.0;
+            const double l_s = in.s != 0.0f ? in.s * exp((static_cast<double>(in.m) - m) * a.inv_t) : 0.0;
+            const double share = r_s / (r_s + l_s), p = fmax(sh.rest_p, 0.0);
+            sh.joined = Joined{m, static_cast<float>(1.0 / (r_s + l_s)), rest.s != 0.0f ? static_cast<float>(1.0 - p / share) : 1.0f,
+                               static_cast<float>(log(r_s + l_s)), rest.s != 0.0f ? static_cast<float>(log(share)) : -CUDART_INF_F};
+        }
+        __syncthreads();
+    }
+    const Joined all = a.tail ? sh.joined : Joined{sh.rest.m, 1.0f / sh.rest.s, 1.0f, logf(sh.rest.s), 0.0f};
 
     // Rows of at most K logits may be listed whole: then there is no rest, whatever rounding leaves of the teacher's sum.
     bool outside = true;
@@ -951,25 +986,19 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const Distill
         for (int k = tid; k < a.K; k += kThreads) distinct += first_of_id(sh, a.K, k, &p) ? 1.0f : 0.0f;
         outside = block_sum(distinct, sh.part) < static_cast<float>(a.V);
     }
-    const float log_s = logf(all.s);
-    const double inv_t = 1.0 / a.temperature;
-    const float p_rest = a.tail ? fmaxf(sh.rest_p, 0.0f) : 0.0f;
-    // log of the rest's share, from its own maximum and sum; nothing there: the share is 0
-    const float log_rest = rest.s != 0.0f ? static_cast<float>((static_cast<double>(rest.m) - all.m) * inv_t) + logf(rest.s / all.s) : -CUDART_INF_F;
-    float factor = 1.0f;
-    if (a.tail && rest.s != 0.0f) factor = 1.0f - p_rest * expf(-log_rest);
+    const float p_rest = a.tail ? static_cast<float>(fmax(sh.rest_p, 0.0)) : 0.0f;
     // a row without any entry has no loss and no gradient
     const bool on = a.tail || sh.total_p != 0.0f;
-    const float4 saved = make_float4(all.m, 1.0f / all.s, factor, on ? 1.0f : 0.0f);
+    const float4 saved = make_float4(all.m, all.inv_s, all.factor, on ? 1.0f : 0.0f);
     if (part == 0) {
         float loss = 0.0f;
         for (int k = tid; k < a.K; k += kThreads) {
             const Entry e = sh.entry[k];
-            if (e.id >= 0 && e.p != 0.0f) loss += e.p * static_cast<float>(e.logp - ((static_cast<double>(e.z) - all.m) * inv_t - log_s));
+            if (e.id >= 0 && e.p != 0.0f) loss += e.p * static_cast<float>(e.logp - ((static_cast<double>(e.z) - all.m) * a.inv_t - all.log_s));
         }
         loss = block_sum(loss, sh.part);
         if (tid == 0) {
-            if (p_rest != 0.0f && outside) loss += p_rest * (logf(p_rest) - log_rest);
+            if (p_rest != 0.0f && outside) loss += p_rest * (logf(p_rest) - all.log_share);
             const float w = a.weights != nullptr ? a.weights[r] : 1.0f;
             a.row_loss[r] = loss * static_cast<float>(a.temperature * a.temperature) * w;
             if (a.saved != nullptr) a.saved[r] = saved;
@@ -1060,7 +1089,7 @@ int launch_distill(const DistillArgs& a, int64_t rows, cudaStream_t stream) {
     const int64_t largest = part_bytes<T>(a.V, least, a.tail != 0, &words);
     if (largest > kPartLimit) return fail(BSI_ERR_UNSUPPORTED, "distill: the bits of a vocabulary of this size do not fit a cluster's shared memory");
     const int per_sm = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kPerSm, kSmShared / (largest + static_cast<int64_t>(sizeof(DistillShared)) + 1024))));
-    const Walk walk = walk_over(rows, a.V, sizeof(T), least, per_sm);
+    const Walk walk = walk_over(rows, a.V, sizeof(T), least, vocab::kMaxCluster, per_sm);
     const int64_t bytes = part_bytes<T>(a.V, walk.parts, a.tail != 0, &words);
     return launch_rows(distill_kernel<T, GRAD>, walk, bytes, stream, "distill", a, words, kStages);
 }
@@ -1156,7 +1185,7 @@ extern "C" int bsi_b200_distill_forward(const void* logits, int dtype, int64_t r
     rc = require_sm100();
     if (rc != BSI_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, factor_of(temperature), temperature, tail != 0, weights, row_loss,
+    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, factor_of(temperature), temperature, 1.0 / temperature, tail != 0, weights, row_loss,
                   reinterpret_cast<float4*>(saved), nullptr, 0, nullptr, nullptr, 0};
     if (rows > 0) {
         rc = dtype == BSI_DTYPE_F32 ? launch_distill<float, false>(a, rows, s)
@@ -1182,7 +1211,7 @@ extern "C" int bsi_b200_distill_backward(const void* logits, int dtype, int64_t 
     rc = require_sm100();
     if (rc != BSI_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, factor_of(temperature), temperature, tail != 0, weights, nullptr,
+    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, factor_of(temperature), temperature, 1.0 / temperature, tail != 0, weights, nullptr,
                   const_cast<float4*>(reinterpret_cast<const float4*>(saved)), upstream, upstream_stride, denominator, grad, grad_stride};
     return dtype == BSI_DTYPE_F32 ? launch_distill_backward<float>(a, rows, s)
            : dtype == BSI_DTYPE_F16 ? launch_distill_backward<__half>(a, rows, s) : launch_distill_backward<__nv_bfloat16>(a, rows, s);
@@ -1206,7 +1235,7 @@ extern "C" int bsi_b200_distill_fused(const void* logits, int dtype, int64_t row
         rc = check_launch("distill weights launch");
         if (rc != BSI_OK) return rc;
     }
-    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, factor_of(temperature), temperature, tail != 0, weights, row_loss,
+    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, factor_of(temperature), temperature, 1.0 / temperature, tail != 0, weights, row_loss,
                   nullptr, nullptr, 0, mean ? weight_sum : nullptr, grad, grad_stride};
     if (rows > 0) {
         rc = dtype == BSI_DTYPE_F32 ? launch_distill<float, true>(a, rows, s)
