@@ -47,29 +47,6 @@ def _reduction(name: str) -> int:
     return _REDUCTIONS[name]
 
 
-class _Distillation(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, ids, teacher, temperature, tail, weights, reduction):
-        loss, saved, total = _ops().distill_forward(logits, ids, teacher, temperature, tail, weights, reduction, True)
-        ctx.save_for_backward(logits, ids, teacher, weights, saved, total)
-        ctx.temperature, ctx.tail = temperature, tail
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, upstream):
-        logits, ids, teacher, weights, saved, total = ctx.saved_tensors
-        grad = _ops().distill_backward(logits, ids, teacher, ctx.temperature, ctx.tail, weights, saved, upstream, total)
-        return grad, None, None, None, None, None, None
-
-
-def _no_gradient(**tensors):
-    if torch.is_grad_enabled():
-        for name, t in tensors.items():
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{name} must not require gradients: the loss is differentiated for the student's logits only")
-
-
 def distillation_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, temperature: float = 1.0, tail: bool = False,
                       weights: Optional[torch.Tensor] = None, reduction: str = "mean") -> torch.Tensor:
     """Kullback-Leibler divergence of the student's ``softmax(logits / temperature)`` from a teacher's top entries, times
@@ -80,11 +57,7 @@ def distillation_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Te
     temperature, and what they leave of 1 is compared with the student's mass outside the list. Entries with an id outside the
     vocabulary are not there; an id listed twice counts with the sum of its probabilities.
     weights: a factor per row, 0 for padding: such a row is not read, its loss and gradient are 0. ``mean`` divides by their sum."""
-    code = _reduction(reduction)
-    _no_gradient(teacher=teacher, weights=weights)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _Distillation.apply(logits, ids, teacher, float(temperature), bool(tail), weights, code)
-    return _ops().distill_forward(logits, ids, teacher, float(temperature), bool(tail), weights, code, False)[0]
+    return _ops().distill_loss(logits, ids, teacher, float(temperature), bool(tail), weights, _reduction(reduction))
 
 
 def distillation_loss_and_grad(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, temperature: float = 1.0, tail: bool = False,

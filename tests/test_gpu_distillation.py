@@ -262,6 +262,26 @@ def test_teacher_in_sixteen_bits_and_ids_in_32():
         check(z, ids, th.float(), w, 1.0, False, loss, x.grad)
 
 
+def test_autograd_s_own_rules():
+    m = scoring()
+    z, ids, t, w = (x.cuda() for x in case(4, 100, 5, torch.float32, False, 1.0, 1))
+    x = z.clone().requires_grad_()
+    loss = m.distillation_loss(x, ids, t)
+    (g,) = torch.autograd.grad(loss, x, retain_graph=True)
+    assert torch.equal(g, torch.autograd.grad(loss, x, retain_graph=True)[0])
+    with pytest.raises(RuntimeError):                     # no second derivative
+        torch.autograd.grad(loss, x, create_graph=True)
+    with torch.no_grad():
+        x.add_(1.0)
+    with pytest.raises(RuntimeError):                     # the logits were changed since
+        loss.backward()
+    with torch.no_grad():
+        assert not m.distillation_loss(x, ids, t).requires_grad
+    y = (z * 2).requires_grad_()                          # behind another operator, and in half a graph
+    (m.distillation_loss(y.half() * 0.5, ids, t, weights=w) * 3).backward()
+    assert y.grad.dtype == torch.float32 and torch.isfinite(y.grad).all() and y.grad.abs().sum() > 0
+
+
 def test_refusals():
     m = scoring()
     z, ids, t, w = (x.cuda() for x in case(4, 100, 5, torch.float32, False, 1.0, 1))
