@@ -455,8 +455,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm) score_kernel(const ScoreArgs
             }
             if (place < a.top) {
                 const float z = vocab::from_ordered(static_cast<uint32_t>(key >> 32));
-                a.top_logprobs[r * a.top + place] = (z - total.m) - log_s;
-                a.top_ids[r * a.top + place] = static_cast<int64_t>(~static_cast<uint32_t>(key));
+                const int64_t at = static_cast<int64_t>(r) * a.top + place;
+                a.top_logprobs[at] = (z - total.m) - log_s;
+                a.top_ids[at] = static_cast<int64_t>(~static_cast<uint32_t>(key));
             }
         }
     }
@@ -560,8 +561,11 @@ RowPlan plan_of(const bsi_row_plan* p) { return RowPlan{p->per, p->block_stride,
 // Entries whose id lies outside the vocabulary are not there. The row's weight and the reduction's factor go on top.
 //
 // With the tail on, what is not listed is summed by itself (a bit per logit says which pieces hold a listed one; such a logit is
-// read as -inf) and the listed ones are added at the end: the rest's mass is no difference of two sums near each other.
-// What a backward pass needs of the forward one is four numbers a row: m, 1 / s, rest's factor, and nothing of the vocabulary's size.
+// read as -inf) and the listed ones are added at the end: the rest's mass is no difference of two sums near each other. With m_out and
+// s_out its own statistics, q_j (1 - rest / q_rest) = exp((z_j - m_out) / T) (q_rest - rest) / s_out: this holds where q_rest is below
+// what a number can be, as where everything outside the list is masked by the type's lowest value.
+// What a backward pass needs of the forward one is four numbers a row: m, 1 / s, (q_rest - rest) / s_out, m_out, and nothing of the
+// vocabulary's size. (Tail off: the third is 1 / s, the last m.)
 
 struct DistillArgs {
     const void* logits;
@@ -577,7 +581,7 @@ struct DistillArgs {
     int tail;
     const float* weights;        // [rows] or null
     float* row_loss;             // [rows], weight and T^2 included
-    float4* saved;               // [rows]: m, 1 / s, factor of q_j outside the list, whether the row is on
+    float4* saved;               // [rows]: see above; 1 / s as -1: the row has no loss
     // gradient
     const float* upstream;       // null: 1
     int64_t upstream_stride;     // 0: one value for all rows
@@ -593,9 +597,10 @@ struct Entry {
     float z;
 };
 
-// A row's softmax: maximum, 1 / sum, the factor of q outside the list, log of the sum, log of what is not listed's share.
+// A row's softmax: maximum, 1 / sum; factor and reference of the exponentials outside the list; log of the sum, log of what is not
+// listed's share.
 struct Joined {
-    float m, inv_s, factor, log_s, log_share;
+    float m, inv_s, factor, ref, log_s, log_share;
 };
 
 struct DistillShared {
@@ -728,7 +733,7 @@ __device__ __forceinline__ bool first_of_id(const DistillShared& sh, int K, int 
     return first;
 }
 
-// The gradient of a part of a row: factor * q_j everywhere, then the listed logits by themselves.
+// The gradient of a part of a row: rest * exp((z_j - ref) / T) everywhere, then the listed logits by themselves.
 template <typename T>
 struct Gradient {
     static constexpr int kVec = Piece<T>::kVec;
@@ -736,19 +741,19 @@ struct Gradient {
     uint4* out_grid;
     vocab::Factor c;
     double inv_t;
-    float m, rest, top, scale;
+    float m, ref, rest, top, scale;
     bool vector, on;
 
     __device__ __forceinline__ Gradient(const DistillArgs& a, uint32_t r, const Span<T>& span, const float4& saved, float s)
-        : out(static_cast<T*>(a.grad) + r * a.grad_stride), c(a.c), inv_t(a.inv_t), m(saved.x), rest(s * saved.z * saved.y), top(s * saved.y),
-          scale(s), vector((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(T) == static_cast<unsigned>(span.shift)), on(saved.w != 0.0f && s != 0.0f) {
+        : out(static_cast<T*>(a.grad) + r * a.grad_stride), c(a.c), inv_t(a.inv_t), m(saved.x), ref(saved.w), rest(s * saved.z), top(s * saved.y),
+          scale(s), vector((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(T) == static_cast<unsigned>(span.shift)), on(!(saved.y < 0.0f) && s != 0.0f) {
         out_grid = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(out) & ~uintptr_t(15));
     }
     __device__ __forceinline__ void write(const Span<T>& span, const uint4& u, int v) const {
         float z[kVec];
         if (on) {
             Piece<T>::unpack(u, z);
-            const vocab::Two less(-m, -m), cc(c.hi, c.hi), ll(c.lo, c.lo), rr(rest, rest);
+            const vocab::Two less(-ref, -ref), cc(c.hi, c.hi), ll(c.lo, c.lo), rr(rest, rest);
 #pragma unroll
             for (int e = 0; e < kVec; e += 2) {
                 float d0, d1;
@@ -845,10 +850,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const Distill
     if (a.weights != nullptr && a.weights[r] == 0.0f) {      // every CTA of the cluster alike: a padded row is not read
         if (part == 0 && tid == 0) {
             a.row_loss[r] = 0.0f;
-            if (a.saved != nullptr) a.saved[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (a.saved != nullptr) a.saved[r] = make_float4(0.0f, -1.0f, 0.0f, 0.0f);
         }
         if (GRAD) {
-            const Gradient<T> g(a, r, span, make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f);
+            const Gradient<T> g(a, r, span, make_float4(0.0f, -1.0f, 0.0f, 0.0f), 0.0f);
             g.write_part(span);
             g.write_ends(span);
         }
@@ -964,20 +969,24 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const Distill
         __syncthreads();
     }
     if (a.tail) {
-        // What is listed and what is not, joined in double by one thread: the gradient of what is not listed goes with 1 - rest / q_rest,
+        // What is listed and what is not, joined in double by one thread: the gradient of what is not listed goes with q_rest - rest,
         // which is small where the teacher's rest and the student's are alike.
         if (tid == 0) {
             const Stats rest = sh.rest, in = sh.listed;
             const float m = vocab::max_nan(rest.m, in.m);
             const double r_s = rest.s != 0.0f ? rest.s * exp((static_cast<double>(rest.m) - m) * a.inv_t) : 0.0;
             const double l_s = in.s != 0.0f ? in.s * exp((static_cast<double>(in.m) - m) * a.inv_t) : 0.0;
-            const double share = r_s / (r_s + l_s), p = fmax(sh.rest_p, 0.0);
-            sh.joined = Joined{m, static_cast<float>(1.0 / (r_s + l_s)), rest.s != 0.0f ? static_cast<float>(1.0 - p / share) : 1.0f,
-                               static_cast<float>(log(r_s + l_s)), rest.s != 0.0f ? static_cast<float>(log(share)) : -CUDART_INF_F};
+            const double total = r_s + l_s, p = fmax(sh.rest_p, 0.0);
+            sh.joined = Joined{m, static_cast<float>(1.0 / total), 0.0f, m, static_cast<float>(log(total)), -CUDART_INF_F};
+            if (rest.s != 0.0f) {
+                sh.joined.factor = static_cast<float>((r_s / total - p) / rest.s);
+                sh.joined.ref = rest.m;
+                sh.joined.log_share = static_cast<float>((static_cast<double>(rest.m) - m) * a.inv_t + log(rest.s / total));
+            }
         }
         __syncthreads();
     }
-    const Joined all = a.tail ? sh.joined : Joined{sh.rest.m, 1.0f / sh.rest.s, 1.0f, logf(sh.rest.s), 0.0f};
+    const Joined all = a.tail ? sh.joined : Joined{sh.rest.m, 1.0f / sh.rest.s, 1.0f / sh.rest.s, sh.rest.m, logf(sh.rest.s), 0.0f};
 
     // Rows of at most K logits may be listed whole: then there is no rest, whatever rounding leaves of the teacher's sum.
     bool outside = true;
@@ -989,7 +998,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const Distill
     const float p_rest = a.tail ? static_cast<float>(fmax(sh.rest_p, 0.0)) : 0.0f;
     // a row without any entry has no loss and no gradient
     const bool on = a.tail || sh.total_p != 0.0f;
-    const float4 saved = make_float4(all.m, all.inv_s, all.factor, on ? 1.0f : 0.0f);
+    const float4 saved = make_float4(all.m, on ? all.inv_s : -1.0f, all.factor, all.ref);
     if (part == 0) {
         float loss = 0.0f;
         for (int k = tid; k < a.K; k += kThreads) {
@@ -1000,7 +1009,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const Distill
         if (tid == 0) {
             if (p_rest != 0.0f && outside) loss += p_rest * (logf(p_rest) - all.log_share);
             const float w = a.weights != nullptr ? a.weights[r] : 1.0f;
-            a.row_loss[r] = loss * static_cast<float>(a.temperature * a.temperature) * w;
+            a.row_loss[r] = static_cast<float>(static_cast<double>(loss) * (a.temperature * a.temperature) * w);      // T^2 alone may pass float32's range
             if (a.saved != nullptr) a.saved[r] = saved;
         }
     }
@@ -1022,7 +1031,7 @@ __global__ void __launch_bounds__(kThreads, 4) distill_backward_kernel(const Dis
     const T* row = static_cast<const T*>(a.logits) + a.rows.at(r);
     const Span<T> span(row, static_cast<int>(a.V), static_cast<int>(blockIdx.x % parts), parts);
     const float4 saved = a.saved[r];
-    if (saved.w != 0.0f && threadIdx.x >= kThreads - 32) {
+    if (!(saved.y < 0.0f) && threadIdx.x >= kThreads - 32) {
         ask_entries(sh, a, r);
         ask_logits<T>(sh, a, row);
         finish_entries<T>(sh, a, r, row);

@@ -31,7 +31,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 struct RowPlan {
     int64_t per, block, row;
     __device__ __forceinline__ int64_t at(uint32_t r) const {      // rows are fewer than 2^31; a 64-bit division costs 100 instructions
-        if (per == 0) return r * row;
+        if (per == 0) return static_cast<int64_t>(r) * row;
         const uint32_t n = static_cast<uint32_t>(per), b = r / n;
         return b * block + (r - b * n) * row;
     }

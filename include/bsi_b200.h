@@ -452,7 +452,8 @@ typedef struct bsi_row_plan {
  * a lower index (0: the argmax), entropy = -sum p log p, and the `top` largest entries, their log probabilities and indices, equal
  * values by ascending index. top at most 128 and V. A token outside [0, V) is not scored: logprob 0, rank -1. A row that holds a NaN or
  * +inf, or nothing but -inf, has NaN for its log probabilities and entropy; its rank means nothing. logprobs, ranks and entropy may
- * be NULL. All outputs are contiguous, [rows] and [rows, top]. */
+ * be NULL. All outputs are contiguous, [rows] and [rows, top]. A wait that gives up, here or in what follows, shows in
+ * bsi_b200_device_status as 144. */
 int bsi_b200_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan,
                             const int64_t* tokens, const bsi_row_plan* token_plan, int top,
                             float* logprobs, int64_t* ranks, float* entropy, float* top_logprobs, int64_t* top_ids,
@@ -465,7 +466,8 @@ int bsi_b200_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t
  * Entries with an id outside [0, V) are not there; an id listed twice counts with the sum of its probabilities. A row's loss is
  * multiplied by weights[r] (float32, NULL: 1); a row of weight 0 is not read, its loss and gradient are 0. loss: the sum over the rows,
  * mean != 0: divided by the weights' sum (0 where that is 0), which weight_sum receives. row_loss [rows]: the rows' weighted losses.
- * saved [rows, 4] float32, 16-byte aligned: what the backward pass takes. loss, weight_sum and saved may be NULL. */
+ * saved [rows, 4] float32, 16-byte aligned: what the backward pass takes. loss, weight_sum and saved may be NULL. temperature: 1e-30 to
+ * 1e30. */
 int bsi_b200_distill_forward(const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan,
                              const int64_t* ids, const void* teacher, int teacher_dtype, int K, double temperature, int tail,
                              const float* weights, int mean, float* row_loss, float* saved, float* loss, float* weight_sum,

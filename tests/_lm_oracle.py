@@ -48,8 +48,9 @@ def distill(z, ids, t, temperature, tail, weight=1.0):
     loss = np.sum(p[on] * (logp[on] - logq[ids[on]]))
     grad = q - p_of
     if tail and not listed.all():
-        out = e[~listed].sum() / e.sum()
+        top = logq[~listed].max()
+        out = np.exp(logq[~listed] - top)            # against its own largest: top + log(sum) has no digits left where top is 1e38
         if rest > 0:
-            loss += rest * (np.log(rest) - np.log(out))
-        grad[~listed] = q[~listed] * (1.0 - rest / out)
+            loss += rest * (np.log(rest) - top - np.log(out.sum()))
+        grad[~listed] = q[~listed] - rest * out / out.sum()
     return weight * T * T * loss, weight * T * grad

@@ -262,6 +262,31 @@ def test_teacher_in_sixteen_bits_and_ids_in_32():
         check(z, ids, th.float(), w, 1.0, False, loss, x.grad)
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("gap", [60.0, 200.0, 5000.0, None])
+def test_everything_outside_the_list_far_below(dtype, gap):
+    """The student's share of what is not listed is below float32's numbers (and float64's); None: masked by the type's lowest value."""
+    dt, T, K = DT[dtype], 2.0, 6
+    z, ids, t, w = case(3, 1003, K, dt, True, T, 21, holes=False)
+    out = torch.ones(3, 1003, dtype=torch.bool).scatter_(1, ids, False)
+    z[out] = torch.finfo(dt).min if gap is None else (z.float() - gap).to(dt)[out]
+    t[:] = torch.log_softmax(torch.cat([t, torch.full((3, 1), -2.0)], 1), -1)[:, :K]        # leaves a rest of some per cent
+    x = z.cuda().requires_grad_()
+    m = scoring()
+    loss = m.distillation_loss(x, ids.cuda(), t.cuda(), T, True, w.cuda(), "none")
+    loss.sum().backward()
+    both = m.distillation_loss_and_grad(z.cuda(), ids.cuda(), t.cuda(), T, True, w.cuda(), "none")
+    for got_loss, got in ((loss.detach(), x.grad), (both[0], both[1])):
+        for r in range(3):
+            want_loss, want = oracle.distill(z[r].double().numpy(), ids[r].numpy(), t[r].double().numpy(), T, True, float(w[r]))
+            # see grad_tolerance: q, p and here rest times its share of what is not listed, each 2e-5 off at most
+            share = w[r].double().numpy() * T * 2e-5 * np.where(out[r].numpy(), 0.0, 3.0) + 2e-5 * np.abs(want)
+            far = np.abs(got[r].double().cpu().numpy() - want) - grad_tolerance(want, 0.0, 1.0, dt) - share
+            assert far.max() <= 0, (r, int(far.argmax()))
+            if want_loss < 3.4e38:
+                assert abs(float(got_loss[r]) - want_loss) <= 2e-5 * (abs(want_loss) + 20 * T * T * float(w[r]))
+
+
 def test_autograd_s_own_rules():
     m = scoring()
     z, ids, t, w = (x.cuda() for x in case(4, 100, 5, torch.float32, False, 1.0, 1))
