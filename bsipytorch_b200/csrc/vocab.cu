@@ -604,11 +604,13 @@ struct Joined {
 };
 
 struct DistillShared {
-    Stats warp[kWarps], warp_listed[kWarps];
+    Stats warp[kWarps];
     float part[kWarps];
+    double listed_part[kWarps];
     vocab::Feed feed;
-    Stats rest, listed;          // of this CTA's part of the row, read by the other CTAs
+    Stats rest;                  // of this CTA's part of the row, read by the other CTAs
     Joined joined;
+    float listed_top;                  // the largest of the logits that the entries name
     double rest_p;                     // what the entries' probabilities leave of 1
     float total_p;                     // their sum
     long long raw_id[kMaxListed];      // as they lie in memory
@@ -658,10 +660,10 @@ template <typename T>
 __device__ void finish_entries(DistillShared& sh, const DistillArgs& a, int64_t r, const T* row) {
     const int lane = threadIdx.x & 31;
     copies_done();
-    float top = -CUDART_INF_F;
+    float top = -CUDART_INF_F, top_z = -CUDART_INF_F;
     for (int k = lane; k < a.K; k += 32) {
         const int id = sh.entry[k].id;
-        float t = -CUDART_INF_F, z = 0.0f;
+        float t = -CUDART_INF_F, z = -CUDART_INF_F;
         if (id >= 0) {
             t = a.teacher_dtype == BSI_DTYPE_F32 ? sh.raw_t[k] : teacher_value(a.teacher, a.teacher_dtype, r * a.K + k);
             const uint32_t word = sh.raw_z[k];
@@ -675,9 +677,13 @@ __device__ void finish_entries(DistillShared& sh, const DistillArgs& a, int64_t 
         sh.entry[k].logp = t;
         sh.entry[k].z = z;
         top = vocab::max_nan(top, t);
+        top_z = vocab::max_nan(top_z, z);
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = vocab::max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    for (int o = 16; o > 0; o >>= 1) {
+        top = vocab::max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        top_z = vocab::max_nan(top_z, __shfl_xor_sync(0xFFFFFFFFu, top_z, o));
+    }
     const double scale = a.tail ? 1.0 : a.inv_t;
     // log p = (t - top) / T - log sum exp((t - top) / T), or t as it is
     const double from = a.tail || top == -CUDART_INF_F ? 0.0 : static_cast<double>(top);
@@ -699,6 +705,7 @@ __device__ void finish_entries(DistillShared& sh, const DistillArgs& a, int64_t 
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     if (lane == 0) {
+        sh.listed_top = top_z;
         sh.total_p = static_cast<float>(sum);
         sh.rest_p = 1.0 - sum;
     }
@@ -733,6 +740,21 @@ __device__ __forceinline__ bool first_of_id(const DistillShared& sh, int K, int 
     return first;
 }
 
+// A warp's share of the listed logits' sum of exponentials against the largest of them, in double and by every CTA for the whole row:
+// they hold most of the mass, and a gradient is the difference of a listed q and its p. (With ex2.approx single entries of
+// 96 x 128011 float32 were off by 5e-4 of the gradient's rms.)
+__device__ __noinline__ double listed_sum(const DistillShared& sh, int K, double inv_t) {
+    double sum = 0.0;
+    for (int k = threadIdx.x; k < K; k += kThreads) {
+        const float z = sh.entry[k].z;
+        float p;
+        if (z != -CUDART_INF_F && first_of_id(sh, K, k, &p)) sum += exp((static_cast<double>(z) - sh.listed_top) * inv_t);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    return sum;
+}
+
 // The gradient of a part of a row: rest * exp((z_j - ref) / T) everywhere, then the listed logits by themselves.
 template <typename T>
 struct Gradient {
@@ -741,11 +763,11 @@ struct Gradient {
     uint4* out_grid;
     vocab::Factor c;
     double inv_t;
-    float m, ref, rest, top, scale;
+    float m, ref, rest, inv_s, scale;
     bool vector, on;
 
     __device__ __forceinline__ Gradient(const DistillArgs& a, uint32_t r, const Span<T>& span, const float4& saved, float s)
-        : out(static_cast<T*>(a.grad) + r * a.grad_stride), c(a.c), inv_t(a.inv_t), m(saved.x), ref(saved.w), rest(s * saved.z), top(s * saved.y),
+        : out(static_cast<T*>(a.grad) + r * a.grad_stride), c(a.c), inv_t(a.inv_t), m(saved.x), ref(saved.w), rest(s * saved.z), inv_s(saved.y),
           scale(s), vector((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(T) == static_cast<unsigned>(span.shift)), on(!(saved.y < 0.0f) && s != 0.0f) {
         out_grid = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(out) & ~uintptr_t(15));
     }
@@ -803,7 +825,7 @@ struct Gradient {
             float p;
             if (!first_of_id(sh, K, k, &p)) continue;
             const double q = exp((static_cast<double>(sh.entry[k].z) - m) * inv_t);
-            out[id] = Piece<T>::narrow(static_cast<float>(top * q - static_cast<double>(scale) * p));
+            out[id] = Piece<T>::narrow(static_cast<float>(scale * (inv_s * q - p)));
         }
     }
 };
@@ -930,25 +952,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const Distill
         if (q < a.count) ask_entries(sh, a, q);
     }
     __syncthreads();
-    Stats listed{-CUDART_INF_F, 0.0f, 0.0f};
     if (a.tail) {
-        for (int k = tid; k < a.K; k += kThreads) {
-            const int id = sh.entry[k].id;
-            float p;
-            if (id >= lo && id < hi && first_of_id(sh, a.K, k, &p)) listed = vocab::merge(listed, Stats{sh.entry[k].z, sh.entry[k].z == -CUDART_INF_F ? 0.0f : 1.0f, 0.0f}, c);
-        }
-        listed = vocab::warp_merge(listed, c);
-        if (lane == 0) sh.warp_listed[warp] = listed;
-        __syncthreads();
+        const double in = listed_sum(sh, a.K, a.inv_t);
+        if (lane == 0) sh.listed_part[warp] = in;
     }
     if (warp == 0) {
-        const Stats none{-CUDART_INF_F, 0.0f, 0.0f};
-        st = vocab::warp_merge(lane < kWarps ? sh.warp[lane] : none, c);
-        if (a.tail) listed = vocab::warp_merge(lane < kWarps ? sh.warp_listed[lane] : none, c);
-        if (lane == 0) {
-            sh.rest = st;
-            sh.listed = listed;
-        }
+        st = vocab::warp_merge(lane < kWarps ? sh.warp[lane] : Stats{-CUDART_INF_F, 0.0f, 0.0f}, c);
+        if (lane == 0) sh.rest = st;
     }
     if (parts > 1) cluster.sync();
     else __syncthreads();
@@ -959,23 +969,21 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const Distill
             const Stats none{-CUDART_INF_F, 0.0f, 0.0f};
             const DistillShared* other = cluster.map_shared_rank(&sh, min(lane, parts - 1));
             st = vocab::warp_merge(lane < parts ? other->rest : none, c);
-            listed = vocab::warp_merge(lane < parts ? other->listed : none, c);
         }
         cluster.sync();      // nobody's shared memory is read by another after this
-        if (tid == 0) {
-            sh.rest = st;
-            sh.listed = listed;
-        }
+        if (tid == 0) sh.rest = st;
         __syncthreads();
     }
     if (a.tail) {
         // What is listed and what is not, joined in double by one thread: the gradient of what is not listed goes with q_rest - rest,
         // which is small where the teacher's rest and the student's are alike.
         if (tid == 0) {
-            const Stats rest = sh.rest, in = sh.listed;
-            const float m = vocab::max_nan(rest.m, in.m);
+            const Stats rest = sh.rest;
+            double in = 0.0;
+            for (int w = 0; w < kWarps; ++w) in += sh.listed_part[w];
+            const float m = vocab::max_nan(rest.m, sh.listed_top);
             const double r_s = rest.s != 0.0f ? rest.s * exp((static_cast<double>(rest.m) - m) * a.inv_t) : 0.0;
-            const double l_s = in.s != 0.0f ? in.s * exp((static_cast<double>(in.m) - m) * a.inv_t) : 0.0;
+            const double l_s = in != 0.0 ? in * exp((static_cast<double>(sh.listed_top) - m) * a.inv_t) : 0.0;
             const double total = r_s + l_s, p = fmax(sh.rest_p, 0.0);
             sh.joined = Joined{m, static_cast<float>(1.0 / total), 0.0f, m, static_cast<float>(log(total)), -CUDART_INF_F};
             if (rest.s != 0.0f) {

@@ -303,19 +303,6 @@ struct Factor {
     __device__ __forceinline__ float times(float x) const { return fmaf(x, lo, x * hi); }
 };
 
-// Two sets of statistics as one.
-__device__ __forceinline__ Stats merge(const Stats& a, const Stats& b, const Factor& c) {
-    Stats r;
-    r.m = max_nan(a.m, b.m);
-    if (r.m == -CUDART_INF_F) return Stats{-CUDART_INF_F, 0.0f, 0.0f};
-    const float da = a.m == -CUDART_INF_F ? 0.0f : c.times(a.m - r.m), db = b.m == -CUDART_INF_F ? 0.0f : c.times(b.m - r.m);
-    const float fa = exp2_fast(da), fb = exp2_fast(db);
-    // a side without any mass adds nothing, however far below it lies
-    r.s = (a.s != 0.0f ? a.s * fa : 0.0f) + (b.s != 0.0f ? b.s * fb : 0.0f);
-    r.w = (a.s != 0.0f && fa != 0.0f ? fa * (a.w + da * a.s) : 0.0f) + (b.s != 0.0f && fb != 0.0f ? fb * (b.w + db * b.s) : 0.0f);
-    return r;
-}
-
 // The warp's statistics as one: their maximum first, then sums against it.
 __device__ __forceinline__ Stats warp_merge(const Stats& v, const Factor& c) {
     float m = v.m;
@@ -543,7 +530,7 @@ struct Running {
         return top;
     }
 
-    // Against m, as merge() takes them.
+    // Against m, as warp_merge() takes them.
     __device__ __forceinline__ Stats stats(const Factor& c) const {
         if (m == -CUDART_INF_F) return Stats{m, 0.0f, 0.0f};
         if (far) return Stats{m, s, w};

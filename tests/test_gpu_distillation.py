@@ -322,3 +322,39 @@ def test_refusals():
                  lambda: m.distillation_loss(z.repeat(1, 10), ids.repeat(1, 120), t.repeat(1, 120))):
         with pytest.raises(RuntimeError):
             call()
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("rows,V", [(64, 20011), (3, 128011)])
+def test_listed_entries_hold_the_mass(tail, rows, V):
+    """Where q and p are both near each other and near 1 in sum, a listed entry's gradient is only as good as the row's total."""
+    K = 16
+    g = torch.Generator().manual_seed(V)
+    z = torch.randn(rows, V, generator=g) - 30.0
+    ids = torch.argsort(torch.rand(rows, V, generator=g), -1)[:, :K]
+    listed = torch.randn(rows, K, generator=g)
+    z.scatter_(1, ids, listed)
+    t = listed + 0.3 * torch.randn(rows, K, generator=g)
+    if tail:
+        t = torch.log_softmax(torch.cat([t, torch.full((rows, 1), -8.0)], 1), -1)[:, :K].contiguous()
+    x = z.cuda().requires_grad_()
+    m = scoring()
+    m.distillation_loss(x, ids.cuda(), t.cuda(), 1.0, tail, reduction="sum").backward()
+    fused = m.distillation_loss_and_grad(z.cuda(), ids.cuda(), t.cuda(), 1.0, tail, reduction="sum")[1]
+    # Scale 1. tail: the listed sum and the total are float64's but for the rest's share (e^-20 of it), then 1 / total, p and the
+    # result are rounded once each. No tail: the total is made of ex2.approx, 2^-22 each for a term and for moving a thread's, a
+    # warp's, a block's and a cluster's sum, and of K additions that are not of next to nothing.
+    total = 2.0 ** -24 if tail else 5 * 2.0 ** -22 + K * 2.0 ** -24
+    for got in (x.grad, fused):
+        got = got.double().cpu().numpy()
+        for r in range(rows):
+            zn, idn = z[r].double().numpy(), ids[r].numpy()
+            _, want = oracle.distill(zn, idn, t[r].double().numpy(), 1.0, tail)
+            q = np.exp(zn - zn.max())
+            q /= q.sum()
+            p = q[idn] - want[idn]
+            far = np.abs(got[r][idn] - want[idn]) - 1.02 * (total * q[idn] + 2.0 ** -24 * (p + np.abs(want[idn])))
+            assert far.max() <= 0, (r, far.max(), got[r][idn][far.argmax()], want[idn][far.argmax()])
+            out = np.ones(V, bool)
+            out[idn] = False      # see grad_tolerance: q, and what p leaves times a logit's share of the rest, which is q's too
+            assert np.all(np.abs(got[r][out] - want[out]) <= 2e-5 * (q[out] + np.abs(want[out])))
