@@ -18,6 +18,7 @@
 // waited for (bounded again), TMEM is freed and the kernel returns.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <math_constants.h>
 
 #include <algorithm>
 
@@ -193,6 +194,15 @@ __device__ __forceinline__ T finished(float sum, float factor, float bias, int r
     return narrow<T>(relu && v < 0.0f ? 0.0f : v);
 }
 
+// The same with the two row factors one after the other, the smaller one first: their product may be infinite where the sum times both
+// is 0 or in range (a token near 3e38 against a weight row near 1e8 that is zero where the token is not: 2^117 * 2^16). With the packer's
+// factors, powers of two from 2^-100 on, and a sum, a multiple of 2^-20, the first step is exact or overflows as the whole does.
+template <typename T>
+__device__ __forceinline__ T finished_apart(float sum, float a, float b, float bias, int relu) {
+    const bool less = fabsf(a) < fabsf(b);
+    return finished<T>(sum * (less ? a : b), less ? b : a, bias, relu);
+}
+
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -358,7 +368,7 @@ __global__ void __launch_bounds__(kThreads) fp4_linear_kernel(const __grid_const
         tc_fence_after();
     }
     auto store = [&](float v, int c) {
-        if (c < a.M && n < a.N) y[c * a.ldy + n] = finished<OutT>(v, gw * token_scale[c], bias, a.relu);
+        if (c < a.M && n < a.N) y[c * a.ldy + n] = finished_apart<OutT>(v, gw, token_scale[c], bias, a.relu);
     };
     if (epi && ok) {
         const uint32_t at = tmem + (static_cast<uint32_t>(quad * 32) << 16);
@@ -653,6 +663,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             for (int c = lane; c < kCols; c += 32) scale[c] = a.x_row != nullptr && m + c < a.M ? *behind_wait(a.x_row + m + c) : 1.0f;
             const float gw = a.w_row != nullptr && n < a.N ? a.w_row[n] : 1.0f, bias = a.bias != nullptr && n < a.N ? a.bias[n] : 0.0f;
             __syncwarp();
+            // The product of two row factors is one instruction less an output than one factor after the other; a warp whose factors could
+            // leave float32's normal numbers together (also a NaN: the largest as a whole number) takes them apart.
+            bool apart = false;
+            if constexpr (!MX) {
+                uint32_t high = 0u, low = 0xFFFFFFFFu;
+                for (int c = lane; c < kCols; c += 32) {
+                    const uint32_t bits = __float_as_uint(fabsf(scale[c]));
+                    high = max(high, bits);
+                    low = min(low, bits);
+                }
+                const uint32_t w = __float_as_uint(fabsf(gw));
+                const float most = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, high)) * __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, w));
+                const float least = __uint_as_float(__reduce_min_sync(0xFFFFFFFFu, low)) * __uint_as_float(__reduce_min_sync(0xFFFFFFFFu, w));
+                apart = !(most < CUDART_INF_F && least >= 1.17549435e-38f);
+            }
             if (!__all_sync(0xFFFFFFFFu, wait(tfull, phase, 6))) break;
             phase ^= 1u;
             tc_fence_after();
@@ -668,7 +693,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             const int tokens = min(kCols, a.M - m);
             if (n < a.N) {
                 OutT* y = static_cast<OutT*>(a.y) + static_cast<int64_t>(m) * a.ldy + n;
-                if (tokens == kCols) {
+                if (apart) {
+                    // seldom: a small loop over a copy in local memory, so that the code around it stays as short as without
+                    float sums[kCols];
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c) sums[c] = __int_as_float(v[c / 32][c % 32]);
+#pragma unroll 1
+                    for (int c = 0; c < tokens; ++c, y += a.ldy) *y = finished_apart<OutT>(sums[c], gw, scale[c], bias, a.relu);
+                } else if (tokens == kCols) {
 #pragma unroll
                     for (int c = 0; c < kCols; ++c, y += a.ldy) *y = finished<OutT>(__int_as_float(v[c / 32][c % 32]), gw * scale[c], bias, a.relu);
                 } else {

@@ -507,7 +507,8 @@ int bsi_b200_fp4_dequantize(const uint8_t* codes, int64_t ld, const uint8_t* sca
                             int format, void* out, int dtype, int64_t ldo, bsi_stream_t stream);
 /* y[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]) of two matrices packed in the same format, x [M, K] and w [N, K]: products and block
  * scales on the tensor cores, float32 sums, one rounding to y_dtype. bias float32 [N] or NULL; activation BSI_ACT_*. row scales are
- * factors of any float32 value. behind_packer != 0: the launch right before this one on the stream is the
+ * factors of the packer's kind (powers of two from 2^-100 on, or NaN), whose product may lie outside float32's range as long as the
+ * result does not. behind_packer != 0: the launch right before this one on the stream is the
  * bsi_b200_fp4_quantize that writes x, and nothing that may still run writes w: w is then read while x is still being packed. A wait
  * that gives up shows in bsi_b200_device_status as 129 to 134. */
 int bsi_b200_fp4_linear(const uint8_t* x_codes, int64_t ldx, const uint8_t* x_scales, const float* x_row_scale,

@@ -172,6 +172,26 @@ def test_a_row_that_is_not_finite(fmt):
     assert torch.isnan(m.quantize_fp4(x.cuda(), fmt).dequantize()[2, 100])
 
 
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("M,N", [(2, 130), (60, 300), (130, 257), (1030, 3500)])
+def test_rows_at_both_ends_of_float32(fmt, M, N):
+    """The factors of a token and of a weight's row are infinite together, or 0, where the sum times both is in range; the narrow kernel
+    and both widths of the paired one."""
+    K = 64
+    x, w = inputs(M, K, torch.float32, M).clamp(-4, 4), (inputs(N, K, torch.float32, N) * 0.05).clamp(-0.2, 0.2)
+    x[0, 0], w[0, :32], w[0, 40] = 3e38, 0.0, 1e8         # 2^117 * 2^16, a sum of 0
+    if fmt == "nvfp4":                                    # 2^-75 * 2^-75, a sum of 64 * 2688^2
+        for r in (1, -1):
+            x[r], w[r] = 2688.0 * 2.0 ** -75, 2688.0 * 2.0 ** -75
+    m = microscale()
+    for bias in (None, torch.linspace(-1, 1, N)):
+        y = m.fp4_linear(x.cuda(), m.quantize_fp4(w.cuda(), fmt), None if bias is None else bias.cuda())
+        assert bool(torch.isfinite(y).all())
+        check_product(x, w, bias, fmt, False, y)
+    # nvfp4: nothing but the bias, as what the token has beside 3e38 is below its row's scales (an mxfp4 block has a scale of its own)
+    assert fmt == "mxfp4" or y[0, 0] == -1.0
+
+
 def test_one_row_without_a_batch_dimension():
     m = microscale()
     w = m.quantize_fp4(torch.randn(70, 96, device="cuda"))
