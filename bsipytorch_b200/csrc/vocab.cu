@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) score_kernel(const ScoreArgs
         all = vocab::warp_merge(all, natural());
         const int n = __reduce_add_sync(0xFFFFFFFFu, lane < kWarps ? sh.warp_ahead[lane] : 0);
         if (lane == 0) {
-            sh.mine = all;
+            sh.mine = ring.gave_up() ? Stats{CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F} : all;
             sh.ahead = n;
         }
     }
@@ -466,6 +466,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) score_kernel(const ScoreArgs
     wanted = wanted_next;
     zt = zt_next;
     }
+    ring.finish();
 }
 
 // CTAs per row and rows under way: as many CTAs as the GPU holds walk over the rows. A row by itself is read at 20 bytes per ns and CTA,
@@ -958,7 +959,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const Distill
     }
     if (warp == 0) {
         st = vocab::warp_merge(lane < kWarps ? sh.warp[lane] : Stats{-CUDART_INF_F, 0.0f, 0.0f}, c);
-        if (lane == 0) sh.rest = st;
+        if (lane == 0) sh.rest = ring.gave_up() ? Stats{CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F} : st;
     }
     if (parts > 1) cluster.sync();
     else __syncthreads();
@@ -1030,6 +1031,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_kernel(const Distill
         if (g.on) g.write_listed(sh, span, a.K);
     }
     }
+    ring.finish();
 }
 
 template <typename T>

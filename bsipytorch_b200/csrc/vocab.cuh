@@ -325,9 +325,15 @@ __device__ __forceinline__ Stats warp_merge(const Stats& v, const Factor& c) {
 // shared memory: chunks of kBatch pieces per thread, copied in bulk by one thread and waited for by all, one row's behind the other's.
 // What is under way depends neither on what the threads hold in registers nor on where in a row they are: a row's first chunks come
 // while the row before it is being finished. As many chunks as there are stages are under way; a stage is filled again when every warp
-// is done with it. Every wait is bounded: one that gives up leaves `broken`, the status word says so, and nothing is waited for any more.
+// is done with it. Every wait is bounded: one that gives up says so in the status word and to the block, which then waits for nothing any
+// more, gives NaN for the row and the rows behind it (gave_up(), behind a barrier of the block), and at the end for what is still under way
+// to land, bounded again: a copy must not arrive in shared memory that has become another CTA's.
+#ifndef BSI_ROWS_WAIT_CYCLES
+#define BSI_ROWS_WAIT_CYCLES 500000000ll       // about 0.25 s; real waits are microseconds
+#define BSI_ROWS_WAIT_HINT 20000u              // ns that a wait may sleep before it looks at the clock; 0: it does not
+#endif
 constexpr int kChunk = kBatch * kThreads;      // pieces
-constexpr long long kWaitCycles = 500000000ll; // about 0.25 s; real waits are microseconds
+constexpr long long kWaitCycles = BSI_ROWS_WAIT_CYCLES;
 
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
@@ -337,9 +343,10 @@ struct Feed {
     const float* weights;
     RowPlan rows;
     int V, part, parts;
-    uint32_t row, step, end, stage;
+    uint32_t row, step, end, stage, round;      // round: how often the stages have been through
     int chunk, pieces;
     const uint4* source;
+    int broken;        // by any thread
 };
 
 // The next row that has pieces, from r on.
@@ -384,7 +391,8 @@ struct Ring {
             f->parts = ps;
             f->step = stride;
             f->end = last_row;
-            f->stage = 0;
+            f->stage = f->round = 0;
+            f->broken = 0;
             open_row<T>(f, first_row);
             for (int i = 0; i < n; ++i) issue();
         }
@@ -399,23 +407,43 @@ struct Ring {
                      ::"r"(shared_address(data + s * kChunk)), "l"(__cvta_generic_to_global(feed->source + at)), "r"(bytes), "r"(full + 8u * s)
                      : "memory");
         feed->stage = s + 1 == stages ? 0u : s + 1;
+        if (s + 1 == stages) ++feed->round;
         ++feed->chunk;
         if (feed->chunk * kChunk >= feed->pieces) open_row<T>(feed, feed->row + feed->step);
     }
-    __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity) {
-        if (broken) return;
-        long long t0 = 0;
-        for (;;) {
-            uint32_t ok;
+    static __device__ __forceinline__ bool landed(uint32_t bar, uint32_t parity) {
+        uint32_t ok;
+        if constexpr (BSI_ROWS_WAIT_HINT == 0u)
+            asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                         : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        else
             asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n"
-                         : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
-            if (ok) return;
-            const long long now = clock64();
-            if (t0 == 0) t0 = now;
-            if (now - t0 > kWaitCycles) {
-                broken = true;
+                         : "=r"(ok) : "r"(bar), "r"(parity), "r"(BSI_ROWS_WAIT_HINT) : "memory");
+        return ok != 0u;
+    }
+    __device__ __forceinline__ bool gave_up() const { return *static_cast<volatile int*>(&feed->broken) != 0; }
+    __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity) {
+        if (!broken && !landed(bar, parity)) broken = !waited(feed, bar, parity, status);
+    }
+    static __device__ __noinline__ bool waited(Feed* feed, uint32_t bar, uint32_t parity, int* status) {
+        const long long t0 = clock64();
+        while (!landed(bar, parity)) {
+            volatile int* gave_up = &feed->broken;
+            if (clock64() - t0 > kWaitCycles) {
+                *gave_up = 1;
                 atomicCAS(status, 0, 144);
-                return;
+            }
+            if (*gave_up != 0) return false;
+        }
+        return true;
+    }
+    // Behind the last row.
+    __device__ __forceinline__ void finish() const {
+        if (threadIdx.x == 0 && gave_up()) {
+            for (uint32_t s = 0; s < stages; ++s) {
+                const uint32_t times = feed->round + (s < feed->stage ? 1u : 0u);      // how often it has been filled
+                const long long t0 = clock64();
+                while (times != 0u && !landed(full + 8u * s, (times - 1u) & 1u) && clock64() - t0 < 30000000ll) {}
             }
         }
     }
