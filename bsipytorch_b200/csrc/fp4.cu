@@ -14,6 +14,7 @@
 // (r % 32) * 16 + (r % 128) / 32 * 4 + j of tile (r / 128, group), groups of 4 consecutive blocks; as many groups as ceil(K / 256) * 256
 // columns have, those behind K zero.
 #include <algorithm>
+#include <type_traits>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -234,12 +235,15 @@ __global__ void __launch_bounds__(256) fp4_dequantize_kernel(const uint8_t* __re
         const int block = i * kVec / (MX ? 32 : 16);
         const uint32_t byte = stile[static_cast<int64_t>(block >> 2) * 512 + (block & 3)];
         const float scale = MX ? (byte == 255u ? __uint_as_float(0x7FC00000u) : power_of_two(static_cast<int>(byte) - 127)) : e4m3_value(byte) * g;
-        // always all eight codes of a word: with the upper half of its bytes unread, the conversions of the lower came out as zeros
-        float v[8];
-        e2m1_values(reinterpret_cast<const uint32_t*>(crow)[i * kVec / 8], v);
+        using Codes = std::conditional_t<kVec == 4, uint16_t, uint32_t>;
+        const uint32_t word = reinterpret_cast<const Codes*>(crow)[i];
         alignas(16) T y[kVec];
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) y[e] = static_cast<T>((kVec == 4 && (i & 1) != 0 ? v[(e + 4) % 8] : v[e]) * scale);
+        for (int e = 0; e < kVec; e += 2) {
+            const float2 v = e2m1_values(word >> (4 * e) & 255u);
+            y[e] = static_cast<T>(v.x * scale);
+            y[e + 1] = static_cast<T>(v.y * scale);
+        }
         const int64_t c = static_cast<int64_t>(i) * kVec;
         if (vector && c + kVec <= K) {
             *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(y);

@@ -70,6 +70,20 @@ def test_codes_and_scales(fmt, dtype, kind, rows, K):
     assert q.shape == (rows, K) and q.dtype == DT[dtype]
 
 
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_every_byte_of_codes_in_every_place(fmt, dtype):
+    """Unpacked values of all 256 bytes at each of 16 neighbouring places, with block scales of 1; a width that ends inside a piece."""
+    m = microscale()
+    grid = np.concatenate([GRID, -GRID])
+    first = m.quantize_fp4(torch.full((256, 32 * 8 - 3), 6.0 if fmt == "nvfp4" else 4.0, device="cuda"), fmt)
+    assert first.block_scales().mul(1.0 if first.row_scale is None else first.row_scale[:, None]).eq(1.0).all()
+    codes = ((torch.arange(256)[:, None] + 37 * torch.arange(128)[None]) % 256).to(torch.uint8)
+    values = np.stack([grid[codes.numpy() & 15], grid[codes.numpy() >> 4]], -1).reshape(256, 256)[:, :253]
+    got = first._replace(codes=codes.cuda()).dequantize(DT[dtype])
+    assert np.array_equal(got.double().cpu().numpy(), values)
+
+
 def test_every_quotient_of_sixteen_bits_beside_the_borders():
     """nvfp4, bfloat16: every value in a block whose largest makes each of the scale's significands."""
     out = []
