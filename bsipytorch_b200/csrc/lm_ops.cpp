@@ -363,8 +363,8 @@ at::Tensor fp4_linear(const torch::Tensor& x, const torch::Tensor& codes, const 
 }
 
 at::Tensor fp4_linear_packed(const torch::Tensor& xc, const torch::Tensor& xs, const OptTensor& xg, const torch::Tensor& codes, const torch::Tensor& scales,
-                             const OptTensor& row_scale, int64_t K, int x_format, int format, const OptTensor& bias, bool relu, py::object dtype) {
-    const Fp4 w(codes, scales, row_scale, K, format), q(xc, xs, xg, K, x_format);
+                             const OptTensor& row_scale, int64_t x_K, int64_t K, int x_format, int format, const OptTensor& bias, bool relu, py::object dtype) {
+    const Fp4 w(codes, scales, row_scale, K, format), q(xc, xs, xg, x_K, x_format);
     c10::cuda::CUDAGuard guard(codes.device());
     return product(q, w, bias_of(bias, w), relu, torch::python::detail::py_object_to_dtype(dtype), false);
 }
@@ -378,7 +378,7 @@ void register_lm_ops(py::module& m) {
     m.def("fp4_linear", &fp4_linear, py::arg("x"), py::arg("codes"), py::arg("scales"), py::arg("row_scale"), py::arg("features"), py::arg("format"),
           py::arg("bias"), py::arg("relu"), py::arg("dtype") = py::none(), "Pack x, then the product with a packed weight");
     m.def("fp4_linear_packed", &fp4_linear_packed, py::arg("x_codes"), py::arg("x_scales"), py::arg("x_row_scale"), py::arg("codes"), py::arg("scales"),
-          py::arg("row_scale"), py::arg("features"), py::arg("x_format"), py::arg("format"), py::arg("bias"), py::arg("relu"), py::arg("dtype"));
+          py::arg("row_scale"), py::arg("x_features"), py::arg("features"), py::arg("x_format"), py::arg("format"), py::arg("bias"), py::arg("relu"), py::arg("dtype"));
     m.def("token_logprobs", &token_logprobs, py::arg("logits"), py::arg("tokens") = py::none(), py::arg("top_k") = 0,
           "(logprobs, ranks, entropy, top_logprobs, top_ids) of rows of logits");
     m.def("distill_loss", &distill_loss, py::arg("logits"), py::arg("ids"), py::arg("teacher"), py::arg("temperature"), py::arg("tail"),

@@ -70,8 +70,8 @@ def fp4_linear(x: Union[torch.Tensor, FP4Matrix], weight: FP4Matrix, bias: Optio
     by default). ``x`` may be packed already (``quantize_fp4``): one packing then serves several weights."""
     f = _format(weight.format)
     if isinstance(x, FP4Matrix):
-        return _ops().fp4_linear_packed(x.codes, x.scales, x.row_scale, weight.codes, weight.scales, weight.row_scale, weight.features,
-                                        _format(x.format), f, bias, relu, out_dtype or x.dtype)
+        return _ops().fp4_linear_packed(x.codes, x.scales, x.row_scale, weight.codes, weight.scales, weight.row_scale, x.features,
+                                        weight.features, _format(x.format), f, bias, relu, out_dtype or x.dtype)
     return _ops().fp4_linear(x, weight.codes, weight.scales, weight.row_scale, weight.features, f, bias, relu, out_dtype)
 
 

@@ -264,3 +264,15 @@ def test_refusals():
                  lambda: m.fp4_linear(x, w._replace(row_scale=None)), lambda: m.fp4_linear(x, w._replace(features=200))):
         with pytest.raises(RuntimeError):
             call()
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_packed_activations_of_another_width_are_refused(fmt):
+    """Also where both widths round up to the same bytes."""
+    m = microscale()
+    w = m.quantize_fp4(torch.randn(64, 50, device="cuda"), fmt)
+    for features in (40, 49, 51, 64, 96):
+        with pytest.raises(RuntimeError, match="features"):
+            m.fp4_linear(m.quantize_fp4(torch.randn(4, features, device="cuda"), fmt), w)
+    x = torch.randn(4, 50, device="cuda")
+    assert torch.equal(m.fp4_linear(m.quantize_fp4(x, fmt), w), m.fp4_linear(x, w))
