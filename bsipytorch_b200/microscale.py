@@ -53,8 +53,9 @@ class FP4Matrix(NamedTuple):
     def block_scales(self) -> torch.Tensor:
         """The block scales as float32 [rows, blocks], without the row scale."""
         rows, blocks = self.codes.shape[0], -(-self.features // _BLOCK[self.format])
-        t = self.scales.view(-(-rows // 128), -1, 32, 4, 4)          # row tile, group, row % 32, row / 32, block
-        t = t.permute(0, 3, 2, 1, 4).reshape(t.shape[0] * 128, -1)[:rows, :blocks].contiguous()
+        groups = -(-self.features // 256) * (256 // _BLOCK[self.format] // 4)
+        t = self.scales.view(-(-rows // 128), groups, 32, 4, 4)      # row tile, group, row % 32, row / 32, block
+        t = t.permute(0, 3, 2, 1, 4).reshape(t.shape[0] * 128, groups * 4)[:rows, :blocks].contiguous()
         return t.view(torch.float8_e8m0fnu if self.format == "mxfp4" else torch.float8_e4m3fn).float()
 
 

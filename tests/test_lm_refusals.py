@@ -101,3 +101,15 @@ def test_names_are_checked_in_python():
         scoring.token_logprobs(torch.zeros(2, 4))
     with pytest.raises(RuntimeError):
         microscale.quantize_fp4(torch.zeros(2, 4))
+
+
+@pytest.mark.parametrize("fmt,block", [("mxfp4", 32), ("nvfp4", 16)])
+@pytest.mark.parametrize("rows,features", [(0, 96), (0, 1), (1, 1), (130, 300)])
+def test_block_scales_of_any_number_of_rows(fmt, block, rows, features):
+    torch = pytest.importorskip("torch")
+    from bsipytorch_b200 import microscale
+    n = capi.lib().bsi_b200_fp4_scale_bytes(rows, features, microscale.FORMATS[fmt])
+    one = torch.full((n,), 127 if fmt == "mxfp4" else 0x38, dtype=torch.uint8)          # 1.0
+    codes = torch.zeros(rows, -(-features // 32) * 16, dtype=torch.uint8)
+    q = microscale.FP4Matrix(codes, one, None, features, fmt, torch.float32)
+    assert torch.equal(q.block_scales(), torch.ones(rows, -(-features // block))) and q.shape == (rows, features)
