@@ -171,19 +171,19 @@ Forward distill_forward(const at::Tensor& logits, const at::Tensor& given_ids, c
     c10::cuda::CUDAGuard guard(z.t.device());
     const Teacher t(z, given_ids, values, weights);
     const at::Device dev = z.t.device();
-    Block block(Block::room(z.rows * 4) + Block::room(z.rows * 16) + 1024, dev);
+    // The loss on an allocation of its own: a caller keeps it long after what the backward pass takes.
     Forward f;
-    at::Tensor row_loss = block.take(z.lead, at::kFloat);
+    f.loss = reduction == kNone ? fresh(z.lead, at::kFloat, dev) : fresh({}, at::kFloat, dev);
+    Block block(Block::room(z.rows * 4) + Block::room(z.rows * 16) + 512, dev);
+    const at::Tensor row_loss = reduction == kNone ? f.loss : block.take(z.lead, at::kFloat);
     if (save) f.saved = block.take({z.rows, 4}, at::kFloat);
-    if (reduction != kNone) f.loss = block.take({}, at::kFloat);
     if (reduction == kMean) f.sum = block.take({}, at::kFloat);
     check_status(bsi_b200_distill_forward(z.t.data_ptr(), z.code, z.rows, z.V, &z.plan, t.ids.data_ptr<int64_t>(), t.values.data_ptr(), t.code, t.K,
                                           temperature, tail ? 1 : 0, t.weight(), reduction == kMean ? 1 : 0,
                                           row_loss.data_ptr<float>(), save ? f.saved.data_ptr<float>() : nullptr,
-                                          f.loss.defined() ? f.loss.data_ptr<float>() : nullptr, f.sum.defined() ? f.sum.data_ptr<float>() : nullptr,
+                                          reduction != kNone ? f.loss.data_ptr<float>() : nullptr, f.sum.defined() ? f.sum.data_ptr<float>() : nullptr,
                                           current_stream()),
                  "bsi_b200_distill_forward");
-    if (reduction == kNone) f.loss = row_loss;
     return f;
 }
 

@@ -358,3 +358,13 @@ def test_listed_entries_hold_the_mass(tail, rows, V):
             out = np.ones(V, bool)
             out[idn] = False      # see grad_tolerance: q, and what p leaves times a logit's share of the rest, which is q's too
             assert np.all(np.abs(got[r][out] - want[out]) <= 2e-5 * (q[out] + np.abs(want[out])))
+
+
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_a_kept_loss_holds_nothing_else(reduction):
+    z, ids, t, w = (x.cuda() for x in case(4096, 64, 5, torch.float32, False, 1.0, 1))
+    x = z.requires_grad_()
+    loss = scoring().distillation_loss(x, ids, t, weights=w, reduction=reduction)
+    loss.sum().backward()
+    kept = loss.detach()
+    assert kept.untyped_storage().nbytes() <= kept.numel() * 4 + 511
