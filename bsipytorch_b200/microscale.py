@@ -50,18 +50,22 @@ class FP4Matrix(NamedTuple):
         """The values that the codes stand for, in ``dtype`` (the packed matrix's own by default)."""
         return _ops().fp4_dequantize(self.codes, self.scales, self.row_scale, self.features, _format(self.format), dtype or self.dtype)
 
+    def _scale_tiles(self) -> torch.Tensor:
+        """A view of the scales: row tile, group of blocks, row % 32, row % 128 / 32, block of the group."""
+        return self.scales.view(-(-self.codes.shape[0] // 128), -(-self.features // 256) * (64 // _BLOCK[self.format]), 32, 4, 4)
+
     def block_scales(self) -> torch.Tensor:
         """The block scales as float32 [rows, blocks], without the row scale."""
         rows, blocks = self.codes.shape[0], -(-self.features // _BLOCK[self.format])
-        groups = -(-self.features // 256) * (256 // _BLOCK[self.format] // 4)
-        t = self.scales.view(-(-rows // 128), groups, 32, 4, 4)      # row tile, group, row % 32, row / 32, block
-        t = t.permute(0, 3, 2, 1, 4).reshape(t.shape[0] * 128, groups * 4)[:rows, :blocks].contiguous()
+        t = self._scale_tiles()
+        t = t.permute(0, 3, 2, 1, 4).reshape(t.shape[0] * 128, t.shape[1] * 4)[:rows, :blocks].contiguous()
         return t.view(torch.float8_e8m0fnu if self.format == "mxfp4" else torch.float8_e4m3fn).float()
 
 
 def quantize_fp4(x: torch.Tensor, format: str = "nvfp4") -> FP4Matrix:
     """Packs ``x`` [..., features] (float32, float16 or bfloat16), leading dimensions as rows. A block (mxfp4) or row (nvfp4) that
-    holds an infinity or a NaN stands for NaN."""
+    holds an infinity or a NaN stands for NaN. The matrix's tensors share one allocation, and the scales' last tile is only written
+    where there are rows."""
     return FP4Matrix(*_ops().fp4_quantize(x, _format(format)), x.shape[-1], format, x.dtype)
 
 
@@ -84,6 +88,11 @@ class FP4Linear(nn.Module):
         self.in_features, self.out_features, self.format = original_linear.in_features, original_linear.out_features, format
         with torch.no_grad():
             packed = quantize_fp4(original_linear.weight.detach(), format)
+        # a copy each, as the packer's outputs share one allocation, and zeros for the scales of rows that are not there, which it
+        # leaves as they were: a buffer can be kept or saved by itself, and equal weights have equal state dicts
+        packed = FP4Matrix(*(t.clone() if isinstance(t, torch.Tensor) else t for t in packed))
+        row = torch.arange(32, device=packed.scales.device)[:, None] + 32 * torch.arange(4, device=packed.scales.device)
+        packed._scale_tiles()[-1:][:, :, row > (self.out_features - 1) % 128] = 0
         self.register_buffer("codes", packed.codes)
         self.register_buffer("scales", packed.scales)
         self.register_buffer("row_scale", packed.row_scale)

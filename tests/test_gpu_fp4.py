@@ -276,3 +276,22 @@ def test_packed_activations_of_another_width_are_refused(fmt):
             m.fp4_linear(m.quantize_fp4(torch.randn(4, features, device="cuda"), fmt), w)
     x = torch.randn(4, 50, device="cuda")
     assert torch.equal(m.fp4_linear(m.quantize_fp4(x, fmt), w), m.fp4_linear(x, w))
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("outputs", [1, 100, 128, 300])
+def test_a_layer_s_buffers(fmt, outputs):
+    """Each on an allocation of its own, with nothing in it that depends on what the memory held before."""
+    m = microscale()
+    lin = torch.nn.Linear(515, outputs, device="cuda")
+    states = []
+    for fill in (0x5A, 0xA5):
+        used = [torch.full((n,), fill, dtype=torch.uint8, device="cuda") for n in [4096] * 64 + [1 << 16] * 64 + [1 << 19] * 16 + [1 << 22]]
+        del used
+        layer = m.FP4Linear(lin, fmt)
+        for b in layer.buffers():
+            assert b.untyped_storage().nbytes() == b.nbytes
+        states.append(layer.state_dict())
+    assert states[0].keys() == states[1].keys() and all(torch.equal(states[0][k], states[1][k]) for k in states[0])
+    x = torch.randn(3, 515, device="cuda")
+    assert torch.equal(layer(x), m.fp4_linear(x, m.quantize_fp4(lin.weight.detach(), fmt), lin.bias.detach()))
