@@ -295,3 +295,19 @@ def test_a_layer_s_buffers(fmt, outputs):
     assert states[0].keys() == states[1].keys() and all(torch.equal(states[0][k], states[1][k]) for k in states[0])
     x = torch.randn(3, 515, device="cuda")
     assert torch.equal(layer(x), m.fp4_linear(x, m.quantize_fp4(lin.weight.detach(), fmt), lin.bias.detach()))
+
+
+# 74 pairs of CTAs walk over tiles of 256 outputs. In order: 70 tiles of 256 tokens, 180 of them (three rounds), 120 tiles of 128 tokens
+# (two rounds, as many as 80 wide ones), the same in one block, 120 tiles of 256 tokens and nine blocks. The ring goes on from one tile
+# to the next out of step with it.
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("M,K,N", [(1030, 515, 3500), (2100, 300, 5003), (384, 1100, 10240), (371, 96, 10235), (1500, 2090, 4999)])
+def test_products_of_more_tiles_than_pairs(fmt, M, K, N):
+    x, w = inputs(M, K, torch.bfloat16, M + K), inputs(N, K, torch.float32, N) * 0.05
+    bias = torch.randn(N, generator=torch.Generator().manual_seed(1)) if N % 2 == 0 else None
+    m = microscale()
+    wq = m.quantize_fp4(w.cuda(), fmt)
+    y = m.fp4_linear(x.cuda(), wq, None if bias is None else bias.cuda(), relu=N % 3 == 0, out_dtype=torch.float32 if K % 2 else None)
+    check_product(x, w, bias, fmt, N % 3 == 0, y)
+    from bsipytorch_b200 import bsi_ops
+    assert bsi_ops.device_status() == 0
