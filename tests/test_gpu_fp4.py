@@ -311,3 +311,17 @@ def test_products_of_more_tiles_than_pairs(fmt, M, K, N):
     check_product(x, w, bias, fmt, N % 3 == 0, y)
     from bsipytorch_b200 import bsi_ops
     assert bsi_ops.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_more_elements_than_32_bits_count(fmt):
+    m = microscale()
+    x = torch.empty(131073, 16400, dtype=torch.bfloat16, device="cuda").normal_(0.0, 1.0, generator=torch.Generator(device="cuda").manual_seed(2))
+    q = m.quantize_fp4(x, fmt)
+    back = q.dequantize()
+    last = m.quantize_fp4(x[-200:], fmt)
+    assert torch.equal(q.codes[-200:], last.codes) and torch.equal(back[-200:], last.dequantize())
+    w = m.quantize_fp4(inputs(140, 16400, torch.float32, 3).cuda(), fmt)
+    y = m.fp4_linear(q, w)
+    assert torch.equal(y[-200:].isfinite().all(), torch.tensor(True, device="cuda"))
+    check_product(x[-3:].cpu(), inputs(140, 16400, torch.float32, 3), None, fmt, False, y[-3:])

@@ -138,3 +138,27 @@ def test_a_tail_over_more_logits_than_a_cluster_has_bits_for():
         scoring().distillation_loss(z, ids, t, tail=True)
     loss = scoring().distillation_loss(z, ids, t)                # without it any length will do: log 12000000, as p is 1
     assert abs(float(loss) - np.log(12e6)) <= (2e-5 + 12e6 / 16384 * 2.0 ** -24) * 37
+
+
+def test_more_logits_than_32_bits_count():
+    rows, V, K = 43001, 50003, 3                     # 2,150,179,003 of them
+    g = torch.Generator(device="cuda").manual_seed(1)
+    z = torch.empty(rows, V, dtype=torch.bfloat16, device="cuda").normal_(0.0, 2.5, generator=g)
+    tokens = torch.randint(0, V, (rows,), generator=g, device="cuda")
+    got = scoring().token_logprobs(z, tokens, top_k=K)
+    some = [0, rows // 2, rows - 60, rows - 1]
+    compare(z[some], tokens[some], type(got)(*(t[some] for t in got)), K)
+    t = got.top_logprobs + 0.1 * torch.randn(rows, K, generator=g, device="cuda")
+    x = z.requires_grad_()
+    scoring().distillation_loss(x, got.top_ids, t, reduction="sum").backward()
+    _, grad = scoring().distillation_loss_and_grad(z.detach(), got.top_ids, t, reduction="sum")
+    for gr in (x.grad, grad):
+        for r in some:
+            zn, idn = z[r].detach().double().cpu().numpy(), got.top_ids[r].cpu().numpy()
+            want = oracle.distill(zn, idn, t[r].double().cpu().numpy(), 1.0, False)[1]
+            q = np.exp(zn - zn.max())
+            q /= q.sum()
+            np.add.at(q, idn, 1.0 / K + 1.0)
+            far = np.abs(gr[r].double().cpu().numpy() - want) - grad_tolerance(want, q, 1.0, torch.bfloat16)
+            assert far.max() <= 0, (r, int(far.argmax()))
+    assert clean()
