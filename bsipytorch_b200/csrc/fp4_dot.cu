@@ -82,7 +82,7 @@ struct Args {
     int M, N;                // tokens, outputs
     int blocks;              // k-blocks
     int relu;
-    int dependent;           // the packer in front may still be running: what it writes is read behind griddepcontrol.wait
+    int dependent;           // launched behind the packer as its dependent: what it writes is read behind griddepcontrol.wait
 };
 
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort_flag, int site) {
@@ -286,7 +286,8 @@ __global__ void __launch_bounds__(kThreads) fp4_linear_kernel(const __grid_const
                 tma_load_2d(dst + C::kWBytes, &map_x, (kb0 + i) * kRowBytes, 0, full(s));
                 bulk_load(dst + C::kWBytes + C::kXBytes + C::kWScale, xs + static_cast<int64_t>(kb0 + i) * C::kXScale, C::kXScale, full(s));
             };
-            // the weights come from before the packer: a ring of them ahead of the wait for it
+            // the weights come from before the packer: a ring of them ahead of the wait for it. (The packer lets nothing start before
+            // its CTAs have exited, so this is ahead of its writes becoming visible, not beside the packing.)
             const int ahead = a.dependent ? min(kStages, count) : 0;
             for (int i = 0; i < ahead; ++i) load_w(i);
             if (a.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -1096,7 +1096,7 @@ int64_t part_bytes(int64_t V, int parts, bool tail, int* bit_words) {
 }
 
 constexpr int64_t kSmShared = 227 * 1024;
-constexpr int kPartLimit = 200 * 1024;      // dynamic shared memory of a CTA, beside about 10 KB of static
+constexpr int kPartLimit = 200 * 1024;      // dynamic shared memory of a CTA, beside 17 KB of static
 
 template <typename T, bool GRAD>
 int launch_distill(const DistillArgs& a, int64_t rows, cudaStream_t stream) {

@@ -207,8 +207,9 @@ class OPTForCausalLM(nn.Module):
 
     def distillation_loss(self, input_ids, ids, teacher, **options):
         """scoring.distillation_loss of this model's next-token logits against a teacher's top entries at the same positions, such as
-        ``top_ids`` and ``top_logprobs`` of the dense model's ``score(input_ids, top_k)`` (with ``tail=True``). Gradients reach the
-        parameters that are still dense; quantised linears pass none on."""
+        ``top_ids`` and ``top_logprobs`` of the dense model's ``score(input_ids, top_k)`` (with ``tail=True``). Quantised linears
+        pass no gradient on: with every linear of the layers quantised, the head and the last norm get theirs, the layers' own norms
+        none, and the embeddings, beside their part as a tied head, what comes down the residual stream past the layers."""
         return distillation_loss(self(input_ids)[:, :-1], ids, teacher, **options)
 
 

@@ -34,7 +34,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
 
     A token outside the vocabulary, such as an ignore index of -100, is not scored: logprob 0, rank -1; its row still has an entropy
     and alternatives. ``tokens=None`` scores none. ``top_k`` is at most 128. A row that holds a NaN or +inf, or nothing but -inf, has
-    NaN log probabilities and entropy. Nothing is recorded for gradients."""
+    NaN log probabilities and entropy. The five tensors share one allocation: one that is kept keeps all. Nothing is recorded for
+    gradients."""
     return TokenLogprobs(*_ops().token_logprobs(logits, tokens, int(top_k)))
 
 
@@ -56,7 +57,8 @@ def distillation_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Te
     log probabilities), renormalised over the listed entries at the temperature. ``tail=True``: it holds log probabilities at the
     temperature, and what they leave of 1 is compared with the student's mass outside the list. Entries with an id outside the
     vocabulary are not there; an id listed twice counts with the sum of its probabilities.
-    weights: a factor per row, 0 for padding: such a row is not read, its loss and gradient are 0. ``mean`` divides by their sum."""
+    weights: a factor per row, 0 for padding: such a row is not read, its loss and gradient are 0. ``mean`` divides by their sum.
+    Vocabularies of up to 2 ** 30; with the tail about 11 million, and a RuntimeError beyond."""
     return _ops().distill_loss(logits, ids, teacher, float(temperature), bool(tail), weights, _reduction(reduction))
 
 

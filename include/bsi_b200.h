@@ -453,7 +453,7 @@ typedef struct bsi_row_plan {
  * values by ascending index. top at most 128 and V. A token outside [0, V) is not scored: logprob 0, rank -1. A row that holds a NaN or
  * +inf, or nothing but -inf, has NaN for its log probabilities and entropy; its rank means nothing. logprobs, ranks and entropy may
  * be NULL. All outputs are contiguous, [rows] and [rows, top]. A wait that gives up, here or in what follows, shows in
- * bsi_b200_device_status as 144. */
+ * bsi_b200_device_status as 144, and the rows that it touched have NaN for their log probabilities, losses and gradients. */
 int bsi_b200_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan,
                             const int64_t* tokens, const bsi_row_plan* token_plan, int top,
                             float* logprobs, int64_t* ranks, float* entropy, float* top_logprobs, int64_t* top_ids,
@@ -467,7 +467,7 @@ int bsi_b200_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t
  * multiplied by weights[r] (float32, NULL: 1); a row of weight 0 is not read, its loss and gradient are 0. loss: the sum over the rows,
  * mean != 0: divided by the weights' sum (0 where that is 0), which weight_sum receives. row_loss [rows]: the rows' weighted losses.
  * saved [rows, 4] float32, 16-byte aligned: what the backward pass takes. loss, weight_sum and saved may be NULL. temperature: 1e-30 to
- * 1e30. */
+ * 1e30. tail 1 takes a bit of shared memory per logit: up to about 11 million logits a row, BSI_ERR_UNSUPPORTED beyond. */
 int bsi_b200_distill_forward(const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan,
                              const int64_t* ids, const void* teacher, int teacher_dtype, int K, double temperature, int tail,
                              const float* weights, int mean, float* row_loss, float* saved, float* loss, float* weight_sum,
@@ -494,9 +494,10 @@ int bsi_b200_distill_fused(const void* logits, int dtype, int64_t rows, int64_t 
  *               magnitude (at least 2^-100; 1 for zeros). row_scale [rows] float32 receives g; a row that holds an infinity or a NaN
  *               gets NaN, and stands for NaN.
  * Elements round to the nearest value, ties to the even code.
- * codes: [rows, ld] bytes, ld a multiple of 16 and at least ceil(K / 32) * 16, zero behind column K. scales: 512 bytes for 128 rows x 4
+ * codes: [rows, ld] bytes, ld a multiple of 16 and at least ceil(K / 32) * 16, zero from column K to there; bytes beyond are not read.
+ * scales: 512 bytes for 128 rows x 4
  * consecutive blocks (row r % 32 at 16 bytes each, then r / 32 % 4 at 4 bytes, then the block), tiles of a row tile behind one
- * another, bsi_b200_fp4_scale_bytes in all (-1 for bad arguments). Both 16-byte aligned. row_scale may be NULL for BSI_FP4_MX. */
+ * another, bsi_b200_fp4_scale_bytes in all (-1 for bad arguments); those of rows that are not there are neither written nor looked at. Both 16-byte aligned. row_scale may be NULL for BSI_FP4_MX. */
 #define BSI_FP4_MX 0
 #define BSI_FP4_NV 1
 int64_t bsi_b200_fp4_scale_bytes(int64_t rows, int64_t K, int format);
@@ -509,8 +510,8 @@ int bsi_b200_fp4_dequantize(const uint8_t* codes, int64_t ld, const uint8_t* sca
  * scales on the tensor cores, float32 sums, one rounding to y_dtype. bias float32 [N] or NULL; activation BSI_ACT_*. row scales are
  * factors of the packer's kind (powers of two from 2^-100 on, or NaN), whose product may lie outside float32's range as long as the
  * result does not. behind_packer != 0: the launch right before this one on the stream is the
- * bsi_b200_fp4_quantize that writes x, and nothing that may still run writes w: w is then read while x is still being packed. A wait
- * that gives up shows in bsi_b200_device_status as 129 to 134. */
+ * bsi_b200_fp4_quantize that writes x, and nothing that may still run writes w: the product is then launched behind the packer's last
+ * CTA and may ask for w before x is visible. A wait that gives up shows in bsi_b200_device_status as 129 to 134. */
 int bsi_b200_fp4_linear(const uint8_t* x_codes, int64_t ldx, const uint8_t* x_scales, const float* x_row_scale,
                         const uint8_t* w_codes, int64_t ldw, const uint8_t* w_scales, const float* w_row_scale, const float* bias,
                         int64_t M, int64_t N, int64_t K, int format, void* y, int64_t ldy, int y_dtype, int activation, int behind_packer,

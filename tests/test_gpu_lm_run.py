@@ -79,3 +79,23 @@ def test_a_bsi_model_is_scored_too():
     logq = torch.log_softmax(logits, -1)
     torch.testing.assert_close(got.logprobs, logq.gather(-1, tokens[:, 1:, None])[..., 0], rtol=0, atol=2e-5)
     assert torch.equal(got.ranks == 0, logits.argmax(-1) == tokens[:, 1:])
+
+
+@pytest.mark.parametrize("quantise", ["fp4", "bsi", "fp4 mlp"])
+def test_what_a_quantised_student_s_gradient_reaches(quantise):
+    from bsipytorch_b200 import microscale
+    student = opt.build_opt_bsi(TINY, dtype=torch.float32) if quantise == "bsi" else opt.build_opt(TINY, dtype=torch.float32, seed=1)
+    if quantise != "bsi":
+        microscale.quantize_model_fp4(student, "nvfp4", scope="mlp" if quantise == "fp4 mlp" else "all", verbose=False)
+    student.requires_grad_(True)
+    tokens = torch.randint(3, TINY.vocab_size, (2, 12), generator=torch.Generator().manual_seed(2)).cuda()
+    with torch.no_grad():
+        answers = student.score(tokens, top_k=8)
+    student.distillation_loss(tokens, answers.top_ids, answers.top_logprobs - 0.1, tail=True).backward()
+    reached = {n for n, p in student.named_parameters() if p.grad is not None and bool(p.grad.any())}
+    want = {"model.decoder.embed_tokens.weight", "model.decoder.embed_positions.weight", "model.decoder.final_layer_norm.weight",
+            "model.decoder.final_layer_norm.bias"}
+    if quantise == "fp4 mlp":          # the attention's projections and the norm in front of them, past the packed half of each layer
+        want |= {n for n, _ in student.named_parameters() if ".self_attn." in n or ".self_attn_layer_norm." in n}
+        reached |= {n for n in want if n.endswith("k_proj.bias")}      # a softmax's gradient for a shift of all its keys is 0
+    assert reached == want
