@@ -550,7 +550,11 @@ int check_rows(const char* what, const void* logits, int dtype, int64_t rows, in
     return BSI_OK;
 }
 
-RowPlan plan_of(const bsi_row_plan* p) { return RowPlan{p->per, p->block_stride, p->row_stride}; }
+// Rows that are all in the first block need no division; what is left of `per` is below the number of rows, 31 bits (a multiple of 2^32 as
+// 32 bits would be a division by 0, and the row it gave no row of the tensor's).
+RowPlan plan_of(const bsi_row_plan* p, int64_t rows) {
+    return p->per >= rows ? RowPlan{0, 0, p->row_stride} : RowPlan{p->per, p->block_stride, p->row_stride};
+}
 
 // ---- distillation from a teacher's top logits ---------------------------------------------------------------------------------
 //
@@ -1177,12 +1181,12 @@ extern "C" int bsi_b200_token_logprobs(const void* logits, int dtype, int64_t ro
         set_error("token_logprobs: top %d, at most %d and the %lld logits of a row", top, kMaxTop, static_cast<long long>(V));
         return BSI_ERR_INVALID;
     }
-    if (tokens != nullptr && token_plan == nullptr) return fail(BSI_ERR_INVALID, "token_logprobs: tokens without a plan");
+    if (tokens != nullptr && (token_plan == nullptr || token_plan->per < 0)) return fail(BSI_ERR_INVALID, "token_logprobs: tokens without a plan");
     if (rows == 0) return BSI_OK;
     if (top > 0 && (top_logprobs == nullptr || top_ids == nullptr)) return fail(BSI_ERR_INVALID, "token_logprobs: null output for the top alternatives");
     rc = require_sm100();
     if (rc != BSI_OK) return rc;
-    ScoreArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, tokens, tokens != nullptr ? plan_of(token_plan) : RowPlan{0, 0, 0}, top,
+    ScoreArgs a{logits, plan_of(plan, rows), static_cast<uint32_t>(rows), V, tokens, tokens != nullptr ? plan_of(token_plan, rows) : RowPlan{0, 0, 0}, top,
                 logprobs, ranks, entropy, top_logprobs, top_ids};
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (dtype) {
@@ -1204,7 +1208,7 @@ extern "C" int bsi_b200_distill_forward(const void* logits, int dtype, int64_t r
     rc = require_sm100();
     if (rc != BSI_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, factor_of(temperature), temperature, 1.0 / temperature, tail != 0, weights, row_loss,
+    DistillArgs a{logits, plan_of(plan, rows), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, factor_of(temperature), temperature, 1.0 / temperature, tail != 0, weights, row_loss,
                   reinterpret_cast<float4*>(saved), nullptr, 0, nullptr, nullptr, 0};
     if (rows > 0) {
         rc = dtype == BSI_DTYPE_F32 ? launch_distill<float, false>(a, rows, s)
@@ -1230,7 +1234,7 @@ extern "C" int bsi_b200_distill_backward(const void* logits, int dtype, int64_t 
     rc = require_sm100();
     if (rc != BSI_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, factor_of(temperature), temperature, 1.0 / temperature, tail != 0, weights, nullptr,
+    DistillArgs a{logits, plan_of(plan, rows), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, factor_of(temperature), temperature, 1.0 / temperature, tail != 0, weights, nullptr,
                   const_cast<float4*>(reinterpret_cast<const float4*>(saved)), upstream, upstream_stride, denominator, grad, grad_stride};
     return dtype == BSI_DTYPE_F32 ? launch_distill_backward<float>(a, rows, s)
            : dtype == BSI_DTYPE_F16 ? launch_distill_backward<__half>(a, rows, s) : launch_distill_backward<__nv_bfloat16>(a, rows, s);
@@ -1254,7 +1258,7 @@ extern "C" int bsi_b200_distill_fused(const void* logits, int dtype, int64_t row
         rc = check_launch("distill weights launch");
         if (rc != BSI_OK) return rc;
     }
-    DistillArgs a{logits, plan_of(plan), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, factor_of(temperature), temperature, 1.0 / temperature, tail != 0, weights, row_loss,
+    DistillArgs a{logits, plan_of(plan, rows), static_cast<uint32_t>(rows), V, ids, teacher, teacher_dtype, K, factor_of(temperature), temperature, 1.0 / temperature, tail != 0, weights, row_loss,
                   nullptr, nullptr, 0, mean ? weight_sum : nullptr, grad, grad_stride};
     if (rows > 0) {
         rc = dtype == BSI_DTYPE_F32 ? launch_distill<float, true>(a, rows, s)

@@ -162,3 +162,30 @@ def test_more_logits_than_32_bits_count():
             far = np.abs(gr[r].double().cpu().numpy() - want) - grad_tolerance(want, q, 1.0, torch.bfloat16)
             assert far.max() <= 0, (r, int(far.argmax()))
     assert clean()
+
+
+@pytest.mark.parametrize("per", [0, 3, 4, 5, (1 << 31) + 1, 1 << 32, (1 << 32) + 2, 3 << 40])
+def test_row_plans_of_any_number_of_rows_per_block(per):
+    """C callers: 5 rows, a block of `per`; with 5 and more the block's stride says nothing."""
+    import ctypes as C
+
+    from bsipytorch_b200 import capi
+
+    class Plan(C.Structure):
+        _fields_ = [("per", C.c_int64), ("block_stride", C.c_int64), ("row_stride", C.c_int64)]
+
+    V, K = 1001, 4
+    z = torch.randn(40, V, device="cuda")
+    at = [r * 2 if per in (0, 5) or per > 5 else r // per * 20 + r % per * 2 for r in range(5)]
+    tokens = torch.randint(0, V, (40,), device="cuda")
+    lp, top, ids = torch.empty(5, device="cuda"), torch.empty(5, K, device="cuda"), torch.empty(5, K, dtype=torch.long, device="cuda")
+    plan, token_plan = Plan(per, 20 * V, 2 * V), Plan(per, 20, 2)
+    capi.check(capi.lib().bsi_b200_token_logprobs(capi.ptr(z), 0, 5, V, C.byref(plan), capi.ptr(tokens), C.byref(token_plan), K, capi.ptr(lp), None, None,
+                                                  capi.ptr(top), capi.ptr(ids), capi.stream_ptr()), "token_logprobs")
+    want = scoring().token_logprobs(z[at], tokens[at], top_k=K)
+    assert torch.equal(ids, want.top_ids)
+    torch.testing.assert_close(lp, want.logprobs, rtol=0, atol=1e-5)
+    each = torch.empty(5, device="cuda")
+    capi.check(capi.lib().bsi_b200_distill_forward(capi.ptr(z), 0, 5, V, C.byref(plan), capi.ptr(ids), capi.ptr(top), 0, K, 1.0, 0, None, 0, capi.ptr(each),
+                                                   None, None, None, capi.stream_ptr()), "distill_forward")
+    torch.testing.assert_close(each, scoring().distillation_loss(z[at], ids, top, reduction="none"), rtol=0, atol=2e-5 * 20)

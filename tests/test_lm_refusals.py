@@ -28,6 +28,8 @@ def test_token_logprobs():
     refused(f(P, 0, 1 << 31, 64, PLAN, P, PLAN, 0, *out, None))
     refused(f(P, 0, 4, 64, None, P, PLAN, 0, *out, None))                 # no plan
     refused(f(P, 0, 4, 64, PLAN, P, None, 0, *out, None))
+    refused(f(P, 0, 4, 64, PLAN, P, C.byref(Plan(-1, 0, 1)), 0, *out, None))
+    refused(f(P, 0, 4, 64, C.byref(Plan(-(1 << 32), 0, 64)), P, PLAN, 0, *out, None))
     refused(f(P, 0, 4, 64, PLAN, P, PLAN, 65, *out, None))                # more alternatives than logits
     refused(f(P, 0, 4, 640, PLAN, P, PLAN, 129, *out, None))
     refused(f(P, 0, 4, 64, PLAN, P, PLAN, 2, P, P, P, None, P, None))     # nowhere to put them
