@@ -269,8 +269,8 @@ int check_matrix(const char* what, int format, int dtype, int64_t rows, int64_t 
         return BSI_ERR_INVALID;
     }
     if (rows > 0 && (codes == nullptr || scales == nullptr || (format == BSI_FP4_NV && row_scale == nullptr) ||
-                     (reinterpret_cast<uintptr_t>(codes) & 15u) || (reinterpret_cast<uintptr_t>(scales) & 15u))) {
-        set_error("%s: null or misaligned codes or scales", what);
+                     (reinterpret_cast<uintptr_t>(codes) & 15u) || (reinterpret_cast<uintptr_t>(scales) & 15u) || (reinterpret_cast<uintptr_t>(row_scale) & 3u))) {
+        set_error("%s: null or misaligned codes, scales or row scales", what);
         return BSI_ERR_INVALID;
     }
     return BSI_OK;

@@ -887,6 +887,8 @@ extern "C" int bsi_b200_fp4_linear(const uint8_t* x_codes, int64_t ldx, const ui
     if (format == BSI_FP4_NV && (x_row_scale == nullptr || w_row_scale == nullptr)) return fail(BSI_ERR_INVALID, "fp4_linear: nvfp4 operands need row scales");
     if ((reinterpret_cast<uintptr_t>(x_codes) | reinterpret_cast<uintptr_t>(w_codes) | reinterpret_cast<uintptr_t>(x_scales) | reinterpret_cast<uintptr_t>(w_scales)) & 15u)
         return fail(BSI_ERR_INVALID, "fp4_linear: codes and scales must be 16-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(x_row_scale) | reinterpret_cast<uintptr_t>(w_row_scale) | reinterpret_cast<uintptr_t>(bias)) & 3u)
+        return fail(BSI_ERR_INVALID, "fp4_linear: misaligned row scales or bias");
     if (reinterpret_cast<uintptr_t>(y) % (y_dtype == BSI_DTYPE_F32 ? 4 : 2) != 0) return fail(BSI_ERR_INVALID, "fp4_linear: misaligned output");
     const int rc = require_sm100();
     if (rc != BSI_OK) return rc;

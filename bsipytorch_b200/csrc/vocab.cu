@@ -529,6 +529,12 @@ int launch_score(const ScoreArgs& a, int64_t rows, cudaStream_t stream) {
 
 constexpr int64_t kMaxRows = 0x7FFFFFFFll / vocab::kMaxCluster;
 
+// Pointers that a kernel reads or writes whole numbers or float32 values through, of `bytes` each.
+template <typename... Pointers>
+bool aligned(uintptr_t bytes, const Pointers*... p) {
+    return (((reinterpret_cast<uintptr_t>(p) % bytes) | ...) == 0);
+}
+
 int check_rows(const char* what, const void* logits, int dtype, int64_t rows, int64_t V, const bsi_row_plan* plan) {
     if (dtype != BSI_DTYPE_F32 && dtype != BSI_DTYPE_F16 && dtype != BSI_DTYPE_BF16) {
         set_error("%s: dtype must be a BSI_DTYPE_* code, got %d", what, dtype);
@@ -1182,6 +1188,7 @@ extern "C" int bsi_b200_token_logprobs(const void* logits, int dtype, int64_t ro
         return BSI_ERR_INVALID;
     }
     if (tokens != nullptr && (token_plan == nullptr || token_plan->per < 0)) return fail(BSI_ERR_INVALID, "token_logprobs: tokens without a plan");
+    if (!aligned(8, tokens, ranks, top_ids) || !aligned(4, logprobs, entropy, top_logprobs)) return fail(BSI_ERR_INVALID, "token_logprobs: misaligned tokens or outputs");
     if (rows == 0) return BSI_OK;
     if (top > 0 && (top_logprobs == nullptr || top_ids == nullptr)) return fail(BSI_ERR_INVALID, "token_logprobs: null output for the top alternatives");
     rc = require_sm100();
@@ -1205,6 +1212,7 @@ extern "C" int bsi_b200_distill_forward(const void* logits, int dtype, int64_t r
     if (rc != BSI_OK) return rc;
     if (rows > 0 && row_loss == nullptr) return fail(BSI_ERR_INVALID, "distill_forward: null row_loss");
     if (reinterpret_cast<uintptr_t>(saved) & 15u) return fail(BSI_ERR_INVALID, "distill_forward: saved must be 16-byte aligned");
+    if (!aligned(4, weights, row_loss, loss, weight_sum)) return fail(BSI_ERR_INVALID, "distill_forward: misaligned weights or outputs");
     rc = require_sm100();
     if (rc != BSI_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -1227,6 +1235,7 @@ extern "C" int bsi_b200_distill_backward(const void* logits, int dtype, int64_t 
     using namespace bsi;
     int rc = check_distill("distill_backward", logits, dtype, rows, V, plan, ids, teacher, teacher_dtype, K, temperature);
     if (rc != BSI_OK) return rc;
+    if (!aligned(4, weights, upstream, denominator)) return fail(BSI_ERR_INVALID, "distill_backward: misaligned weights, upstream or denominator");
     if (rows == 0) return BSI_OK;
     if (saved == nullptr || grad == nullptr || grad_stride < V || (reinterpret_cast<uintptr_t>(saved) & 15u) ||
         reinterpret_cast<uintptr_t>(grad) % (dtype == BSI_DTYPE_F32 ? 4 : 2) != 0)
@@ -1250,6 +1259,7 @@ extern "C" int bsi_b200_distill_fused(const void* logits, int dtype, int64_t row
     if (loss == nullptr || weight_sum == nullptr || (rows > 0 && (row_loss == nullptr || grad == nullptr || grad_stride < V)) ||
         reinterpret_cast<uintptr_t>(grad) % (dtype == BSI_DTYPE_F32 ? 4 : 2) != 0)
         return fail(BSI_ERR_INVALID, "distill_fused: null output, or gradient rows shorter than the vocabulary");
+    if (!aligned(4, weights, row_loss, loss, weight_sum)) return fail(BSI_ERR_INVALID, "distill_fused: misaligned weights or outputs");
     rc = require_sm100();
     if (rc != BSI_OK) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -115,3 +115,35 @@ def test_block_scales_of_any_number_of_rows(fmt, block, rows, features):
     codes = torch.zeros(rows, -(-features // 32) * 16, dtype=torch.uint8)
     q = microscale.FP4Matrix(codes, one, None, features, fmt, torch.float32)
     assert torch.equal(q.block_scales(), torch.ones(rows, -(-features // block))) and q.shape == (rows, features)
+
+
+def test_misaligned_pointers():
+    """A kernel would fault on them."""
+    odd, four = C.c_void_p(258), C.c_void_p(260)
+    f = capi.lib().bsi_b200_token_logprobs
+    refused(f(P, 0, 4, 64, PLAN, four, PLAN, 2, P, P, P, P, P, None))
+    for i, bad in enumerate((odd, four, odd, odd, four)):
+        out = [P] * 5
+        out[i] = bad
+        refused(f(P, 0, 4, 64, PLAN, P, PLAN, 2, *out, None))
+    g, b, h = (getattr(capi.lib(), "bsi_b200_distill_" + n) for n in ("forward", "backward", "fused"))
+    head = (P, 0, 4, 64, PLAN, P, P, 0, 5, 1.0, 0)
+    for i in (0, 2, 4, 5):
+        args = [P, 1, P, P, P, P]
+        args[i] = odd
+        refused(g(*head, *args, None))
+    for i in (0, 2, 4):
+        args = [P, P, P, 1, P, P, 64]
+        args[i] = odd
+        refused(b(*head, *args, None))
+    for i in (0, 2, 3, 4):
+        args = [P, 1, P, P, P, P, 64]
+        args[i] = odd
+        refused(h(*head, *args, None))
+    L = capi.lib()
+    refused(L.bsi_b200_fp4_quantize(P, 0, 4, 64, 64, 1, P, 32, P, odd, None))
+    refused(L.bsi_b200_fp4_dequantize(P, 32, P, odd, 4, 64, 1, P, 0, 64, None))
+    for i in (0, 1, 2):
+        a = [P, P, P]
+        a[i] = odd
+        refused(L.bsi_b200_fp4_linear(P, 32, P, a[0], P, 32, P, a[1], a[2], 4, 8, 64, 1, P, 8, 0, 0, 0, None))
