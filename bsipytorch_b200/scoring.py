@@ -55,7 +55,8 @@ def distillation_loss(logits: torch.Tensor, ids: torch.Tensor, teacher: torch.Te
 
     ids, teacher: [..., entries] with the logits' leading shape, 1 to 512 entries a row. ``tail=False``: ``teacher`` holds logits (or
     log probabilities), renormalised over the listed entries at the temperature. ``tail=True``: it holds log probabilities at the
-    temperature, and what they leave of 1 is compared with the student's mass outside the list. Entries with an id outside the
+    temperature, and what they leave of 1 is compared with the student's mass outside the list (also what rounding leaves: where the
+    list holds all that the teacher gives anything to and the student masks everything else, ``tail=False`` is the loss). Entries with an id outside the
     vocabulary are not there; an id listed twice counts with the sum of its probabilities.
     weights: a factor per row, 0 for padding: such a row is not read, its loss and gradient are 0. ``mean`` divides by their sum.
     Vocabularies of up to 2 ** 30; with the tail about 11 million, and a RuntimeError beyond."""
